@@ -418,6 +418,128 @@ int sv_attn_append_at_peer(sv_kv* kv, int layer, const void* q, int q_type, cons
                            int head_offset, int n_head_total, int slot, int wait_slot, const int32_t* epoch_dev,
                            void* stream);
 
+/* ================================================================ paged 8-bit cache
+ * Many sessions in one pool of fixed-size pages (the reference reserves n_ctx rows per session,
+ * attention.hpp:25-46, and caps a batch at eight, vc3_batch.inc:113; no counterpart there).  A page
+ * holds page_size consecutive tokens of one request for one layer.  Codes are signed 8-bit,
+ * [n_pages][n_kv_head][page_size][head_dim], with one f32 scale for each page and kv head,
+ * [n_pages][n_kv_head]: value = code * scale, codes in [-127, 127].  One scale per page and head
+ * factors out of the dot products, so codes enter the tensor cores as exact f16 integers.
+ *
+ * All memory is the caller's: the store of each layer (sv_paged), and one step's arrays with their
+ * work space (sv_paged_step), which every layer of the step uses.  A step is planned once
+ * (sv_paged_plan), then each layer appends (sv_paged_append) and attends (sv_paged_attn).  Calls of one
+ * step run on one stream (they share its work space); the host reads nothing back, so a step of
+ * fixed bounds is capturable in a CUDA graph.
+ * head_dim 64, 128 or 256; page_size 16, 32, 64 or 128; n_req <= 4096. */
+#define SV_PAGED_MAX_REQ 4096
+#define SV_DEVERR_STEP 8    /* lengths outside the step's bounds (n_new > max_new, more than n_tokens in all): cut */
+#define SV_DEVERR_PAGES 16  /* a token had no page (free list empty, table full, entry out of range): dropped */
+
+typedef struct sv_paged {
+    void* k;              /* int8 [n_pages][n_kv_head][page_size][head_dim], 16-byte aligned */
+    void* v;
+    float* k_scale;       /* f32 [n_pages][n_kv_head] */
+    float* v_scale;
+    int n_pages, n_kv_head, page_size, head_dim;
+    int* err;             /* device error word (SV_DEVERR_* bits are ORed in), or NULL */
+} sv_paged;
+
+typedef struct sv_paged_step {
+    int n_req;            /* requests (rows of `table`) */
+    int n_tokens;         /* rows of this step's q/k/v: an upper bound on the sum of n_new */
+    int max_new;          /* an upper bound on every n_new */
+    int max_blocks;       /* row length of `table`: pages a request may hold */
+    int n_head, n_kv_head, head_dim, page_size, n_pages;
+    const int32_t* n_past;  /* device [n_req]: tokens each request holds before the step */
+    const int32_t* n_new;   /* device [n_req]: tokens it brings (0: none) */
+    int32_t* table;         /* device [n_req][max_blocks]: page of each block; entries of new pages are written */
+    int32_t* q_start;       /* out, device [n_req + 1]: first row of each request */
+    int32_t* kv_len;        /* out, device [n_req]: tokens held after the step */
+    int32_t* tok_req;       /* out, device [n_tokens]: request of each row (-1 past the last) */
+    int32_t* tok_pos;       /* out, device [n_tokens]: position in the request */
+    int32_t* tok_slot;      /* out, device [n_tokens]: page * page_size + offset, or -1 (dropped) */
+    void* work;             /* device, sv_paged_step_bytes(step) bytes, 256-byte aligned */
+    size_t work_bytes;
+    int* err;               /* device error word or NULL */
+} sv_paged_step;
+
+/* Bytes of `work` for a step of these bounds (the pointers are not looked at); 0 if they are refused. */
+size_t sv_paged_step_bytes(const sv_paged_step* step);
+
+/* Block tables, slot map and positions of a step, from request lengths.  With ps = page_size, request r
+ * holds ceil(n_past/ps) pages and needs ceil((n_past + n_new)/ps); the pages that it lacks come off the
+ * top of the free list in request order (the j-th page taken in the step is
+ * free_pages[*n_free - 1 - j]) and are written into its row of `table`.  *n_free_out gets what is left
+ * (another word than n_free).  Running it again on the same inputs gives the same result.  A token
+ * without a page gets slot -1 and kv_len ends before it (SV_DEVERR_PAGES).  A last page that is
+ * partly filled must belong to one request alone. */
+int sv_paged_plan(const sv_paged_step* step, const int32_t* free_pages, const int32_t* n_free, int32_t* n_free_out,
+                  void* stream);
+
+/* Gives the pages of n requests back: for each i < n the ceil(kv_len[i]/page_size) first entries of row
+ * req[i] of `table` are pushed on the free list, in order, and set to -1; *n_free grows by as many.
+ * All device arrays; req without repeats.  free_pages has room for n_pages entries (a push past that is
+ * left out and raises SV_DEVERR_PAGES). */
+int sv_paged_release(int32_t* table, int n_req, int max_blocks, int page_size, int n_pages, const int32_t* req, int n,
+                     const int32_t* kv_len, int32_t* free_pages, int32_t* n_free, int* err, void* stream);
+
+/* Rotary positions.  A pair turns by pos * f_i, f_i = freq_base^(-2i / n_dims) for i < n_dims / 2, the
+ * rotated dims being the first n_dims of a head (any even number up to head_dim); pairs are
+ * (i, i + n_dims/2) for SV_ROPE_NEOX and SV_ROPE_IMROPE and (2i, 2i + 1) for SV_ROPE_NORM.  Long contexts:
+ * freq_factors (host, [n_dims/2], or NULL) divides each f_i; freq_scale (1 = none) stretches positions
+ * by 1/freq_scale, and with ext_factor > 0 the pairs that turn more than beta_fast times in n_ctx_orig
+ * tokens keep f_i, those that turn less than beta_slow times take freq_scale * f_i, and between them the
+ * two are blended linearly in i (YaRN); then cos and sin are also scaled by
+ * attn_factor * (1 + 0.1 ln(1/freq_scale)), else by attn_factor. */
+#define SV_ROPE_NORM 1
+typedef struct sv_rope_params {
+    int mode;              /* SV_ROPE_NORM, SV_ROPE_NEOX or SV_ROPE_IMROPE */
+    int n_dims;
+    int sections[4];       /* IMROPE: see sv_rope */
+    double freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow;  /* f32 would move a long context's angles */
+    int n_ctx_orig;
+    const float* freq_factors;
+} sv_rope_params;
+typedef struct sv_rope_table sv_rope_table;
+/* The frequencies of these parameters, laid out on the device once for all calls. */
+int sv_rope_table_create(int device, const sv_rope_params* p, sv_rope_table** out);
+int sv_rope_table_destroy(sv_rope_table* t);
+
+/* One layer's rows of a planned step, between the QKV projection and the attention: RMSNorm of q and k
+ * per head (norm weights NULL = none), rotary positions of both (rope NULL = none), the rotated queries
+ * to q_out, K and V quantised into the step's pages.  A page's scale is max(s_old, amax/127) over its new
+ * rows, s_old being its scale where it holds earlier rows; if it grows, the codes that it holds are
+ * rounded to it (round-half-even in f32 throughout).  The largest magnitude is taken over finite
+ * values; an infinity is stored as +-127, a NaN as 0, and a page whose values are all below 2^-100 as zeros.
+ * Rows past the last token are not read or written. */
+typedef struct sv_paged_rows {
+    const void *q, *k, *v;     /* device [n_tokens] rows of n_head | n_kv_head x head_dim elements, heads packed */
+    int type;                  /* SV_TYPE_F16 or SV_TYPE_F32 */
+    size_t q_nb, k_nb, v_nb;   /* bytes from a token's row to the next (multiples of 16, pointers too) */
+    const float *q_norm, *k_norm;  /* device [head_dim] or NULL */
+    float eps;
+    const sv_rope_table* rope;
+    const int32_t* pos;        /* device [n_tokens] positions ([4][n_tokens] for IMROPE), or NULL: the step's tok_pos */
+    void* q_out;               /* device [n_tokens][n_head][head_dim]; may be q itself when type and layout agree */
+    int q_out_type;            /* SV_TYPE_F16 or SV_TYPE_F32 */
+} sv_paged_rows;
+int sv_paged_append(const sv_paged* kv, const sv_paged_step* step, const sv_paged_rows* rows, void* stream);
+
+/* Rows of the cache as numbers: k_out and v_out [n][n_kv_head][head_dim] of out_type (F16 or F32) get
+ * code * scale of slots[i]; a slot outside the pool gives zeros and raises SV_DEVERR_ROW_RANGE
+ * (-1: zeros only). */
+int sv_paged_read(const sv_paged* kv, const int32_t* slots, int n, void* k_out, void* v_out, int out_type, void* stream);
+
+/* Causal grouped-query attention of the step's rows over the pages: row t of request r at position p sees
+ * the keys max(0, p - window + 1) .. min(p, kv_len - 1) (window <= 0: from 0).  q: device rows of n_head x
+ * head_dim (F16 or F32, heads packed, q_nb bytes apart; 16-byte aligned), out: [n_tokens][n_head][head_dim] of
+ * out_type (F16 or F32).  A row that sees no key gets zeros; rows past the last token are not written.
+ * F32 queries are rounded to f16.  Requests of few rows (n_new * n_head/n_kv_head <= 16) and of many take
+ * different kernels, with their key ranges split over the SMs by the plan. */
+int sv_paged_attn(const sv_paged* kv, const sv_paged_step* step, const void* q, int q_type, size_t q_nb, float scale,
+                  int window, void* out, int out_type, void* stream);
+
 /* ================================================================ failure detection
  * Every on-device wait of the library is bounded; on expiry the kernel sets
  * SV_DEVERR_TIMEOUT in its error word and unwinds instead of hanging.  This

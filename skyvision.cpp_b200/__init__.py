@@ -14,6 +14,8 @@ interface for this path:
 * ``Session``     -> Qwen3VL's session bookkeeping: window eviction + compaction
                      (qwen3vl_model.cpp:1110-1124, moss_vl_model.cpp:264-291).
 * ``can_splice``  -> the KV splice predicate (qwen3vl_model.cpp:1165-1171).
+* ``PagedKv``, ``PagedStep``, ``Rope`` -> the paged 8-bit cache of many sessions: page plan, rotary
+                     append and attention (no counterpart in the reference).
 
 Device memory, streams and process groups come from PyTorch; the C ABI only
 sees raw pointers and sizes.  There is no CPU fallback: if libsvkv.so is
@@ -34,7 +36,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "svkv.h")
 
 TYPE_F32, TYPE_F16, TYPE_Q8_0 = 0, 1, 8
 MASK_NONE, MASK_CAUSAL, MASK_WINDOW, MASK_EXPLICIT = 0, 1, 2, 3
-DEVERR_ROW_RANGE, DEVERR_TIMEOUT, DEVERR_SEGMENT = 1, 2, 4
+DEVERR_ROW_RANGE, DEVERR_TIMEOUT, DEVERR_SEGMENT, DEVERR_STEP, DEVERR_PAGES = 1, 2, 4, 8, 16
 OK = 0
 STATUS = {0: "ok", -1: "invalid", -2: "unsupported", -3: "cuda", -4: "nomem", -5: "overflow",
           -6: "workspace", -7: "device"}
@@ -70,7 +72,7 @@ class _Rope(ctypes.Structure):
                 ("sections", ctypes.c_int * 4)]
 
 
-ROPE_NONE, ROPE_NEOX, ROPE_IMROPE = 0, 2, 40
+ROPE_NONE, ROPE_NORM, ROPE_NEOX, ROPE_IMROPE = 0, 1, 2, 40
 
 
 class _FaParams(ctypes.Structure):
@@ -82,6 +84,35 @@ class _FaParams(ctypes.Structure):
         ("scale", ctypes.c_float), ("max_bias", ctypes.c_float), ("logit_softcap", ctypes.c_float),
         ("dst", ctypes.c_void_p),
     ]
+
+
+class _Paged(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_int), ("n_kv_head", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("head_dim", ctypes.c_int), ("err", ctypes.c_void_p)]
+
+
+class _PagedStep(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_req", "n_tokens", "max_new", "max_blocks", "n_head", "n_kv_head",
+                                            "head_dim", "page_size", "n_pages")] + \
+               [(n, ctypes.c_void_p) for n in ("n_past", "n_new", "table", "q_start", "kv_len", "tok_req", "tok_pos",
+                                               "tok_slot", "work")] + \
+               [("work_bytes", ctypes.c_size_t), ("err", ctypes.c_void_p)]
+
+
+class _PagedRows(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int),
+                ("q_nb", ctypes.c_size_t), ("k_nb", ctypes.c_size_t), ("v_nb", ctypes.c_size_t),
+                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("rope", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+                ("q_out_type", ctypes.c_int)]
+
+
+class _RopeParams(ctypes.Structure):
+    _fields_ = [("mode", ctypes.c_int), ("n_dims", ctypes.c_int), ("sections", ctypes.c_int * 4)] + \
+               [(n, ctypes.c_double) for n in ("freq_base", "freq_scale", "ext_factor", "attn_factor", "beta_fast",
+                                              "beta_slow")] + \
+               [("n_ctx_orig", ctypes.c_int), ("freq_factors", ctypes.c_void_p)]
 
 
 def lib() -> ctypes.CDLL:
@@ -136,6 +167,14 @@ def lib() -> ctypes.CDLL:
         "sv_out_proj_peer": (I, [P, P, I, ctypes.c_int64, P, I, I, I, I, I, I, P, P, P, P]),
         "sv_peer_destroy": (I, [P]),
         "sv_attn_append_at_peer": (I, [P, I, P, I, P, P, I, I, P, I, F, P, I, I, I, I, P, P]),
+        "sv_paged_step_bytes": (SZ, [ctypes.POINTER(_PagedStep)]),
+        "sv_paged_plan": (I, [P, P, P, P, P]),
+        "sv_paged_release": (I, [P, I, I, I, I, P, I, P, P, P, P, P]),
+        "sv_rope_table_create": (I, [I, ctypes.POINTER(_RopeParams), ctypes.POINTER(P)]),
+        "sv_rope_table_destroy": (I, [P]),
+        "sv_paged_append": (I, [P, P, P, P]),
+        "sv_paged_read": (I, [P, P, I, P, P, I, P]),
+        "sv_paged_attn": (I, [P, P, P, I, SZ, F, I, P, I, P]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -333,6 +372,209 @@ class KvCache:
         f = ctypes.c_int()
         _check("sv_kv_error", lib().sv_kv_error(self.h, ctypes.byref(f), _stream(stream)))
         return f.value
+
+
+# =================================================================== paged 8-bit cache
+def _float_type(fn: str, t) -> int:
+    """SV type id of an f16 or f32 tensor."""
+    import torch
+    if t.dtype == torch.float16:
+        return TYPE_F16
+    if t.dtype == torch.float32:
+        return TYPE_F32
+    raise SvError(fn, -2)
+
+
+def _packed(t, heads: int, hd: int) -> bool:
+    """[T, heads, hd] with a token's heads side by side."""
+    return t.dim() == 3 and t.shape[1] == heads and t.shape[2] == hd and t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd)
+
+
+def _row_bytes(t) -> int:
+    """Bytes from a token's row to the next (one row: its own length)."""
+    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]) * t.element_size()
+
+
+def _require(fn: str, ok) -> None:
+    """A tensor that the library cannot read as it stands is refused like a bad argument."""
+    if not ok:
+        raise SvError(fn, -1)
+
+
+class Rope:
+    """Frequencies of rotary positions, laid out on the device once (sv_rope_table_create).
+
+    mode ROPE_NEOX (pairs i, i + n_dims/2), ROPE_NORM (pairs 2i, 2i + 1) or ROPE_IMROPE (NEOX pairs,
+    `sections`); n_dims even, the rotated part of the head.  Long contexts: freq_scale (1/4 stretches
+    positions by four), ext_factor > 0 with n_ctx_orig for the YaRN blend, or freq_factors."""
+
+    def __init__(self, n_dims: int, mode: int = ROPE_NEOX, freq_base: float = 1e4, freq_scale: float = 1.0,
+                 ext_factor: float = 0.0, attn_factor: float = 1.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 n_ctx_orig: int = 0, freq_factors=None, sections=(0, 0, 0, 0), device: int = 0):
+        self.h = None
+        ff = None if freq_factors is None else np.ascontiguousarray(freq_factors, dtype=np.float32)
+        _require("sv_rope_table_create", ff is None or ff.size == n_dims // 2)
+        p = _RopeParams(mode, n_dims, (ctypes.c_int * 4)(*sections), freq_base, freq_scale, ext_factor, attn_factor,
+                        beta_fast, beta_slow, n_ctx_orig, None if ff is None else ff.ctypes.data)
+        h = ctypes.c_void_p()
+        _check("sv_rope_table_create", lib().sv_rope_table_create(device, ctypes.byref(p), ctypes.byref(h)))
+        self.h, self.mode, self.n_dims = h.value, mode, n_dims
+
+    def free(self) -> None:
+        if self.h:
+            lib().sv_rope_table_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class PagedStep:
+    """One step of a batch of requests over the paged cache: its arrays and work space, for steps of up to
+    n_req requests, n_tokens rows and max_new rows per request.  plan() fills q_start, kv_len, tok_req,
+    tok_pos, tok_slot and n_free on the device; every layer of the step then uses them."""
+
+    def __init__(self, n_req: int, n_tokens: int, max_new: int, page_size: int, n_pages: int, n_head: int,
+                 n_kv_head: int, head_dim: int, device: int = 0):
+        import torch
+        self._s = s = _PagedStep(n_req, n_tokens, max_new, 1, n_head, n_kv_head, head_dim, page_size, n_pages)
+        self._ref = ctypes.byref(s)
+        s.work_bytes = lib().sv_paged_step_bytes(self._ref)
+        if s.work_bytes == 0:
+            raise SvError("sv_paged_step_bytes", -2)
+        dev = torch.device("cuda", device)
+        new = lambda n: torch.zeros(n, dtype=torch.int32, device=dev)  # noqa: E731
+        self.q_start, self.kv_len, self.n_free, self.err = new(n_req + 1), new(n_req), new(1), new(1)
+        self.tok_req, self.tok_pos, self.tok_slot = new(n_tokens), new(n_tokens), new(n_tokens)
+        self.work = torch.empty(s.work_bytes, dtype=torch.uint8, device=dev)
+        for name in ("q_start", "kv_len", "tok_req", "tok_pos", "tok_slot", "work", "err"):
+            setattr(s, name, getattr(self, name).data_ptr())
+        self.n_req, self.n_tokens, self.n_head, self.n_kv_head, self.head_dim = n_req, n_tokens, n_head, n_kv_head, head_dim
+
+    def plan(self, n_past, n_new, table, free_pages, n_free, stream=None) -> None:
+        """Page tables, slot map and work lists of the step (sv_paged_plan): n_past, n_new int32 [n_req],
+        table int32 [n_req, max_blocks] (new pages are written into it), free_pages int32 with *n_free pages.
+        self.n_free gets what is left of them."""
+        import torch
+        i32 = torch.int32
+        _require("sv_paged_plan", n_past.dtype == n_new.dtype == table.dtype == free_pages.dtype == n_free.dtype == i32
+                 and table.is_contiguous() and n_past.is_contiguous() and n_new.is_contiguous()
+                 and free_pages.is_contiguous() and table.dim() == 2 and table.shape[0] == self.n_req
+                 and n_past.numel() == n_new.numel() == self.n_req)
+        s = self._s
+        s.max_blocks = table.shape[1]
+        s.n_past, s.n_new, s.table = n_past.data_ptr(), n_new.data_ptr(), table.data_ptr()
+        self._keep = (n_past, n_new, table)
+        _check("sv_paged_plan", lib().sv_paged_plan(self._ref, free_pages.data_ptr(), n_free.data_ptr(),
+                                                    self.n_free.data_ptr(), _stream(stream)))
+
+    def error_flags(self) -> int:
+        """DEVERR_* bits raised by plans of this step since the last call (waits for them)."""
+        f = int(self.err.item())
+        if f:
+            self.err.zero_()
+        return f
+
+
+class PagedKv:
+    """Pool of n_pages pages of page_size tokens for every layer: signed 8-bit codes
+    [n_pages, n_kv_head, page_size, head_dim] with one f32 scale for each page and kv head (sv_paged)."""
+
+    def __init__(self, n_layer: int, n_kv_head: int, head_dim: int, page_size: int, n_pages: int, device: int = 0):
+        import torch
+        dev = torch.device("cuda", device)
+        self.n_layer, self.n_kv_head, self.head_dim, self.page_size, self.n_pages = n_layer, n_kv_head, head_dim, page_size, n_pages
+        self._codes = torch.zeros((n_layer, 2, n_pages, n_kv_head, page_size, head_dim), dtype=torch.int8, device=dev)
+        self._scales = torch.zeros((n_layer, 2, n_pages, n_kv_head), dtype=torch.float32, device=dev)
+        self.err = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._l = [_Paged(self._codes[i, 0].data_ptr(), self._codes[i, 1].data_ptr(), self._scales[i, 0].data_ptr(),
+                          self._scales[i, 1].data_ptr(), n_pages, n_kv_head, page_size, head_dim, self.err.data_ptr())
+                   for i in range(n_layer)]
+        self._refs = [ctypes.byref(x) for x in self._l]
+
+    def codes(self, layer: int, is_v: bool):
+        """torch int8 view [n_pages, n_kv_head, page_size, head_dim] of a layer's K or V codes."""
+        return self._codes[layer, int(is_v)]
+
+    def scales(self, layer: int, is_v: bool):
+        """torch f32 view [n_pages, n_kv_head] of their scales."""
+        return self._scales[layer, int(is_v)]
+
+    def rope_append(self, layer: int, step: PagedStep, q, k, v, rope: Rope | None = None, q_norm=None, k_norm=None,
+                    eps: float = 1e-6, pos=None, q_out=None, stream=None):
+        """q/k RMSNorm, rotary positions, K/V quantised into the step's pages (sv_paged_append): q [T, n_head, HD],
+        k and v [T, n_kv_head, HD], all f16 or all f32, heads packed, any token stride of 16-byte multiples
+        (views of one projection's output).  pos: int32 [T] ([4, T] for ROPE_IMROPE), or None: the plan's
+        positions.  Returns the rotated queries (f16 unless q_out is given)."""
+        import torch
+        fn, T = "sv_paged_append", step.n_tokens
+        if q_out is None:
+            q_out = torch.empty((T, step.n_head, step.head_dim), dtype=torch.float16, device=q.device)
+        hd = self.head_dim
+        _require(fn, q.shape == (T, step.n_head, hd) and k.shape == v.shape == (T, self.n_kv_head, hd) and q_out.shape == q.shape
+                 and q.dtype == k.dtype == v.dtype and q_out.is_contiguous()
+                 and _packed(q, step.n_head, hd) and _packed(k, self.n_kv_head, hd) and _packed(v, self.n_kv_head, hd)
+                 and (pos is None or (pos.dtype == torch.int32 and pos.is_contiguous()
+                                      and pos.numel() == (4 * T if rope is not None and rope.mode == ROPE_IMROPE else T)))
+                 and all(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == hd)
+                         for w in (q_norm, k_norm)))
+        r = _PagedRows(q.data_ptr(), k.data_ptr(), v.data_ptr(), _float_type(fn, q), _row_bytes(q), _row_bytes(k),
+                       _row_bytes(v), _ptr(q_norm), _ptr(k_norm), eps, None if rope is None else rope.h, _ptr(pos),
+                       q_out.data_ptr(), _float_type(fn, q_out))
+        _check(fn, lib().sv_paged_append(self._refs[layer], step._ref, ctypes.byref(r), _stream(stream)))
+        return q_out
+
+    def read(self, layer: int, slots, k_out=None, v_out=None, stream=None):
+        """Rows of the cache as numbers (sv_paged_read): slots int32 [n] (page * page_size + offset) ->
+        k, v [n, n_kv_head, head_dim], f16 unless outputs are given."""
+        import torch
+        fn = "sv_paged_read"
+        shape = (slots.numel(), self.n_kv_head, self.head_dim)
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=torch.float16, device=slots.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=k_out.dtype, device=slots.device)
+        _require(fn, slots.dtype == torch.int32 and slots.is_contiguous() and k_out.shape == v_out.shape == shape
+                 and k_out.dtype == v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous())
+        _check(fn, lib().sv_paged_read(self._refs[layer], slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
+                                       _float_type(fn, k_out), _stream(stream)))
+        return k_out, v_out
+
+    def attn(self, layer: int, step: PagedStep, q, scale: float, window: int = 0, out=None, stream=None):
+        """Causal attention of the step's rows q [T, n_head, HD] (f16/f32, heads packed) over the pages
+        (sv_paged_attn); window > 0: the last `window` positions only.  Returns [T, n_head, HD] f16 unless
+        out is given."""
+        import torch
+        fn = "sv_paged_attn"
+        if out is None:
+            out = torch.empty((step.n_tokens, step.n_head, step.head_dim), dtype=torch.float16, device=q.device)
+        _require(fn, q.shape == out.shape == (step.n_tokens, step.n_head, self.head_dim)
+                 and _packed(q, step.n_head, self.head_dim) and out.is_contiguous())
+        _check(fn, lib().sv_paged_attn(self._refs[layer], step._ref, q.data_ptr(), _float_type(fn, q),
+                                       _row_bytes(q), scale, window, out.data_ptr(),
+                                       _float_type(fn, out), _stream(stream)))
+        return out
+
+    def release(self, table, req, kv_len, free_pages, n_free, stream=None) -> None:
+        """Pages of the requests `req` (rows of table, holding kv_len[i] tokens) back to the free list
+        (sv_paged_release)."""
+        import torch
+        fn = "sv_paged_release"
+        _require(fn, all(t.dtype == torch.int32 and t.is_contiguous() for t in (table, req, kv_len, free_pages, n_free))
+                 and req.numel() == kv_len.numel() and free_pages.numel() >= self.n_pages)
+        _check(fn, lib().sv_paged_release(table.data_ptr(), table.shape[0], table.shape[1], self.page_size, self.n_pages,
+                                          req.data_ptr(), req.numel(), kv_len.data_ptr(), free_pages.data_ptr(),
+                                          n_free.data_ptr(), self.err.data_ptr(), _stream(stream)))
+
+    def error_flags(self) -> int:
+        """DEVERR_* bits raised since the last call (waits for the work before it)."""
+        f = int(self.err.item())
+        if f:
+            self.err.zero_()
+        return f
 
 
 PEER_HANDLE_BYTES = 64

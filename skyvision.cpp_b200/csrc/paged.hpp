@@ -1,0 +1,83 @@
+// paged.hpp - the paged 8-bit cache: layout of a step's work space and the kernels' launchers.
+//
+// A step is planned once on the device (paged_plan.cu) and used by every layer's append
+// (paged_append.cu) and attention (paged_decode.cu, paged_prefill.cu).  What the layers need from the
+// plan stands in the step's work space, laid out here from the step's host-known bounds alone, so
+// the host never reads anything back:
+//   head      counts of the lists below
+//   req       int4 per request: first row, rows, tokens held before, tokens held after
+//   page      int4 per page that the step writes to: first row, page, first offset, rows
+//   dec       int2 per decode item: request, split | splits << 16
+//   pre       int4 per prefill item: request, query tile, split, splits
+//   tickets   arrival counters of the split merges (zeroed by the plan, and again by each merge)
+//   *_part    unnormalised outputs of the splits; *_ml their running maximum and sum
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/svkv.h"
+#include "internal.hpp"
+
+namespace svkv {
+
+constexpr int kDecRows = 16;      // query rows of one decode unit (the M of its MMA)
+constexpr int kDecTile = 64;      // keys per decode tile
+// decode CTAs that one SM holds (shared memory: a ring of K and V tiles each)
+constexpr int dec_ctas_per_sm(int hd) { return hd == 256 ? 2 : 3; }
+constexpr int pre_rows(int hd) { return hd == 256 ? 128 : 256; }   // query rows of one prefill unit
+constexpr int pre_tile(int hd) { return hd == 256 ? 64 : 128; }    // keys per prefill tile
+// a split shorter than this costs more in its start and merge than it saves
+constexpr int kDecMinTiles = 2;
+constexpr int kPreMinTiles = 4;
+
+enum : int { PH_PAGES = 0, PH_DEC = 1, PH_PRE = 2 };
+
+struct StepLayout {
+    int page_cap = 0, dec_cap = 0, pre_cap = 0;     // most entries of each list
+    int dec_slots = 1, pre_slots = 1;               // items that run at once, per kv head
+    size_t head = 0, req = 0, page = 0, dec = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
+    size_t bytes = 0;
+    int n_ticks = 0;
+};
+
+// false: bounds that this build refuses
+bool step_layout(const sv_paged_step& s, StepLayout* l);
+
+struct RopeTable {
+    int device = 0, mode = 0, n_dims = 0;
+    float mag = 1.0f;
+    float4* pairs = nullptr;    // device [n_dims / 2]: turns per position (high and low part), axis of the position
+};
+
+cudaError_t launch_paged_plan(const sv_paged_step& s, const StepLayout& l, const int32_t* free_pages,
+                              const int32_t* n_free, int32_t* n_free_out, cudaStream_t st);
+cudaError_t launch_paged_release(int32_t* table, int n_req, int max_blocks, int ps, int n_pages, const int32_t* req,
+                                 int n, const int32_t* kv_len, int32_t* free_pages, int32_t* n_free, int* err,
+                                 cudaStream_t st);
+cudaError_t launch_paged_append(const sv_paged& kv, const sv_paged_step& s, const StepLayout& l,
+                                const sv_paged_rows& r, cudaStream_t st);
+cudaError_t launch_paged_read(const sv_paged& kv, const int32_t* slots, int n, void* k_out, void* v_out, int out_type,
+                              cudaStream_t st);
+struct PagedAttn {
+    sv_paged kv;
+    const int32_t* table;
+    int max_blocks;
+    int n_req, n_tokens, n_head, G;
+    const uint8_t* q;
+    int q_type;
+    size_t q_nb;
+    float scale_log2;
+    int window;
+    void* out;
+    int out_type;
+    uint8_t* work;
+    StepLayout l;
+    int* err;
+};
+cudaError_t launch_paged_decode(const PagedAttn& a, cudaStream_t st);
+cudaError_t launch_paged_prefill(const PagedAttn& a, cudaStream_t st);
+
+}  // namespace svkv
+
+struct sv_rope_table : svkv::RopeTable {};

@@ -1,0 +1,136 @@
+// paged_api.cpp - the extern "C" boundary of the paged 8-bit cache: argument checks and launches.
+// Everything the kernels index by is checked here against the host-known bounds; what only the device
+// knows (lengths, table entries, slots) the kernels bound themselves.
+#include <cmath>
+#include <cstdio>
+
+#include "paged.hpp"
+
+using namespace svkv;
+
+namespace {
+
+int status_of(cudaError_t e) {
+    if (e == cudaSuccess) return SV_OK;
+    fprintf(stderr, "svkv: CUDA error %s\n", cudaGetErrorString(e));
+    return SV_ERR_CUDA;
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+bool f16_or_f32(int type) { return type == SV_TYPE_F16 || type == SV_TYPE_F32; }
+
+int check_store(const sv_paged* kv) {
+    if (!kv || !kv->k || !kv->v || !kv->k_scale || !kv->v_scale || kv->n_pages < 1 || kv->n_kv_head < 1) return SV_ERR_INVALID;
+    if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || !aligned(kv->k_scale, 4) || !aligned(kv->v_scale, 4)) return SV_ERR_INVALID;
+    const int ps = kv->page_size, hd = kv->head_dim;
+    if (ps != 16 && ps != 32 && ps != 64 && ps != 128) return SV_ERR_UNSUPPORTED;
+    if (hd != 64 && hd != 128 && hd != 256) return SV_ERR_UNSUPPORTED;
+    if ((int64_t)kv->n_pages * ps > INT32_MAX || kv->n_kv_head > 1024) return SV_ERR_UNSUPPORTED;
+    return SV_OK;
+}
+
+int check_step(const sv_paged_step* s, StepLayout* l) {
+    if (!s || !s->n_past || !s->n_new || !s->table || !s->q_start || !s->kv_len || !s->tok_req || !s->tok_pos || !s->tok_slot ||
+        !s->work)
+        return SV_ERR_INVALID;
+    if (s->n_req < 1 || s->n_tokens < 1 || s->max_new < 1 || s->max_blocks < 1 || s->n_pages < 1 || s->n_head < 1 ||
+        s->n_kv_head < 1)
+        return SV_ERR_INVALID;
+    if (!step_layout(*s, l)) return SV_ERR_UNSUPPORTED;
+    if (!aligned(s->work, 256)) return SV_ERR_INVALID;
+    return s->work_bytes < l->bytes ? SV_ERR_WORKSPACE : SV_OK;
+}
+
+int check_both(const sv_paged* kv, const sv_paged_step* s, StepLayout* l) {
+    if (const int rc = check_store(kv)) return rc;
+    if (const int rc = check_step(s, l)) return rc;
+    return kv->n_kv_head == s->n_kv_head && kv->head_dim == s->head_dim && kv->page_size == s->page_size &&
+                   kv->n_pages == s->n_pages
+               ? SV_OK
+               : SV_ERR_INVALID;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sv_paged_step_bytes(const sv_paged_step* step) {
+    StepLayout l;
+    return step && step_layout(*step, &l) ? l.bytes : 0;
+}
+
+int sv_paged_plan(const sv_paged_step* step, const int32_t* free_pages, const int32_t* n_free, int32_t* n_free_out,
+                  void* stream) {
+    StepLayout l;
+    if (!free_pages || !n_free || !n_free_out || n_free == n_free_out) return SV_ERR_INVALID;
+    if (const int rc = check_step(step, &l)) return rc;
+    return status_of(launch_paged_plan(*step, l, free_pages, n_free, n_free_out, static_cast<cudaStream_t>(stream)));
+}
+
+int sv_paged_release(int32_t* table, int n_req, int max_blocks, int page_size, int n_pages, const int32_t* req, int n,
+                     const int32_t* kv_len, int32_t* free_pages, int32_t* n_free, int* err, void* stream) {
+    if (!table || !req || !kv_len || !free_pages || !n_free || n_req < 1 || max_blocks < 1 || n_pages < 1 || n < 0 || n > n_req)
+        return SV_ERR_INVALID;
+    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128) return SV_ERR_UNSUPPORTED;
+    if (n == 0) return SV_OK;
+    return status_of(launch_paged_release(table, n_req, max_blocks, page_size, n_pages, req, n, kv_len, free_pages, n_free, err,
+                                          static_cast<cudaStream_t>(stream)));
+}
+
+int sv_paged_append(const sv_paged* kv, const sv_paged_step* step, const sv_paged_rows* r, void* stream) {
+    StepLayout l;
+    if (const int rc = check_both(kv, step, &l)) return rc;
+    if (!r || !r->q || !r->k || !r->v || !r->q_out || !(r->eps >= 0.0f)) return SV_ERR_INVALID;
+    if (!f16_or_f32(r->type) || !f16_or_f32(r->q_out_type)) return SV_ERR_UNSUPPORTED;
+    const size_t es = r->type == SV_TYPE_F32 ? 4 : 2, hd = (size_t)step->head_dim;
+    if (!aligned(r->q, 16) || !aligned(r->k, 16) || !aligned(r->v, 16) || !aligned(r->q_out, 16) || ((r->q_nb | r->k_nb | r->v_nb) & 15))
+        return SV_ERR_INVALID;
+    if (r->q_nb < step->n_head * hd * es || r->k_nb < step->n_kv_head * hd * es || r->v_nb < step->n_kv_head * hd * es)
+        return SV_ERR_INVALID;
+    if (r->q_out == r->q && (r->type != r->q_out_type || r->q_nb != step->n_head * hd * es)) return SV_ERR_INVALID;
+    if (r->rope) {
+        if (r->rope->n_dims > step->head_dim) return SV_ERR_INVALID;
+        if (r->rope->mode == SV_ROPE_IMROPE && !r->pos) return SV_ERR_INVALID;
+    }
+    return status_of(launch_paged_append(*kv, *step, l, *r, static_cast<cudaStream_t>(stream)));
+}
+
+int sv_paged_read(const sv_paged* kv, const int32_t* slots, int n, void* k_out, void* v_out, int out_type, void* stream) {
+    if (const int rc = check_store(kv)) return rc;
+    if (n < 0 || (n > 0 && (!slots || !k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16)))) return SV_ERR_INVALID;
+    if (!f16_or_f32(out_type)) return SV_ERR_UNSUPPORTED;
+    if (n == 0) return SV_OK;
+    return status_of(launch_paged_read(*kv, slots, n, k_out, v_out, out_type, static_cast<cudaStream_t>(stream)));
+}
+
+int sv_paged_attn(const sv_paged* kv, const sv_paged_step* step, const void* q, int q_type, size_t q_nb, float scale,
+                  int window, void* out, int out_type, void* stream) {
+    StepLayout l;
+    if (const int rc = check_both(kv, step, &l)) return rc;
+    if (!q || !out || !(scale > 0.0f) || !std::isfinite(scale)) return SV_ERR_INVALID;
+    if (!f16_or_f32(q_type) || !f16_or_f32(out_type)) return SV_ERR_UNSUPPORTED;
+    const size_t es = q_type == SV_TYPE_F32 ? 4 : 2;
+    if (!aligned(q, 16) || !aligned(out, 16) || (q_nb & 15) || q_nb < (size_t)step->n_head * step->head_dim * es) return SV_ERR_INVALID;
+    PagedAttn a{};
+    a.kv = *kv;
+    a.table = step->table;
+    a.max_blocks = step->max_blocks;
+    a.n_req = step->n_req;
+    a.n_tokens = step->n_tokens;
+    a.n_head = step->n_head;
+    a.G = step->n_head / step->n_kv_head;
+    a.q = static_cast<const uint8_t*>(q);
+    a.q_type = q_type;
+    a.q_nb = q_nb;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.window = window > 0 ? window : 0;
+    a.out = out;
+    a.out_type = out_type;
+    a.work = static_cast<uint8_t*>(step->work);
+    a.l = l;
+    a.err = kv->err;
+    return status_of(launch_paged_decode(a, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,365 @@
+// paged_plan.cu - a step's page tables, slot map and work lists, from request lengths.
+//
+// Per request r with p tokens held and n new ones (page size ps): it holds ceil(p/ps) pages and wants
+// ceil((p+n)/ps); q_start, the pages taken before r and the pages touched before r are exclusive prefix
+// sums over the requests.  Every block scans all requests (at most 4096, in shared memory; a scan is
+// cheaper than a second launch or a wait between blocks) and then does its own part: block 0 the
+// per-request outputs and the attention's work lists, the others one row of the step per thread, found
+// by binary search in q_start.  A row whose position starts a page is the one that writes the table's
+// new entry and the step's page record, so there are no atomics and the order is fixed.
+//
+// Bound: latency (a launch, two dependent loads, the scans); the step's arrays are a few hundred KB.
+#include "common.cuh"
+#include "paged.hpp"
+
+namespace svkv {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRowsPerBlock = 512;
+
+struct PlanArgs {
+    sv_paged_step s;
+    StepLayout l;
+    const int32_t *free_pages, *n_free;
+    int32_t* n_free_out;
+    int G, ps_log2;
+};
+
+// exclusive prefix sum over the block's threads; *total gets the sum
+template <class T>
+__device__ __forceinline__ T block_scan(T x, T* total, T* buf) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T v = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();                       // buf may still be read by the scan before
+    if (lane == 31) buf[warp] = v;
+    __syncthreads();
+    T before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; w++) {
+        if (w < warp) before += buf[w];
+        all += buf[w];
+    }
+    *total = all;
+    return before + v - x;
+}
+
+// last i in [0, n) with start[i] <= x (start non-decreasing, start[0] = 0)
+__device__ __forceinline__ int find_last(const int* start, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Splits of units so that their items fill `slots` once: the shortest piece length (in tiles) that gives
+// no more than `slots` items, but at least min_tiles.  cost(u): tiles of unit u (0: not a unit).
+template <class Cost>
+__device__ int piece_of(int n_units, int slots, int min_tiles, Cost cost, long long* buf) {
+    long long sum = 0, total;
+    for (int u = threadIdx.x; u < n_units; u += kThreads) sum += cost(u);
+    block_scan<long long>(sum, &total, buf);
+    long long piece = (total + slots - 1) / slots;
+    if (piece < min_tiles) piece = min_tiles;
+    for (int it = 0; it < 8; it++) {
+        long long n = 0, all;
+        for (int u = threadIdx.x; u < n_units; u += kThreads) n += (cost(u) + piece - 1) / piece;
+        block_scan<long long>(n, &all, buf);
+        if (all <= slots) break;
+        const long long next = (piece * all + slots - 1) / slots;
+        if (next >= total) {
+            piece = total > min_tiles ? total : min_tiles;
+            break;
+        }
+        piece = next > piece ? next : piece + 1;
+    }
+    return (int)piece;
+}
+
+__global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_constant__ PlanArgs a) {
+    extern __shared__ int sm[];
+    __shared__ long long buf[kThreads / 32];
+    const sv_paged_step& s = a.s;
+    const int n = s.n_req, ps = s.page_size, lg = a.ps_log2;
+    int* start = sm;                   // [n + 1] first row of each request
+    int* past = start + n + 1;         // [n]
+    int* taken = past + n;             // [n + 1] pages taken before r
+    int* touched = taken + n + 1;      // [n + 1] pages written to before r
+    int* tiles = touched + n + 1;      // [n + 1] prefill query tiles before r
+    pdl_wait();
+    const int per = (n + kThreads - 1) / kThreads;
+    const int r0 = min(n, (int)threadIdx.x * per), r1 = min(n, r0 + per);
+    const int nf = min(max(__ldg(a.n_free), 0), s.n_pages);
+    int err = 0;
+    {
+        int sum = 0;
+        for (int r = r0; r < r1; r++) {
+            const int x = __ldg(s.n_new + r), p = __ldg(s.n_past + r);
+            const int c = min(max(x, 0), s.max_new);
+            if (c != x || p < 0 || (p + ps - 1) >> lg > s.max_blocks) err |= SV_DEVERR_STEP;
+            past[r] = min(max(p, 0), s.max_blocks << lg);
+            start[r] = c;
+            sum += c;
+        }
+        long long total;
+        long long at = block_scan<long long>(sum, &total, buf);
+        for (int r = r0; r < r1; r++) {
+            const int c = start[r];
+            start[r] = (int)min(at, (long long)s.n_tokens);
+            at += c;
+        }
+        if (total > s.n_tokens) err |= SV_DEVERR_STEP;
+        if (threadIdx.x == 0) start[n] = (int)min(total, (long long)s.n_tokens);
+    }
+    __syncthreads();
+    const int rows_per_unit = pre_rows(s.head_dim);
+    {
+        // pages taken and pages touched are below 2^31 each: scanned as the two halves of one word
+        unsigned long long sum = 0;
+        int tl = 0;
+        auto of = [&](int r, int* np, int* nt, int* ql) {
+            const int p = past[r], c = start[r + 1] - start[r];
+            const int held = (p + ps - 1) >> lg, want = min((p + c + ps - 1) >> lg, s.max_blocks);
+            *np = max(want - held, 0);
+            *nt = c > 0 ? ((p + c - 1) >> lg) - (p >> lg) + 1 : 0;
+            *ql = c * a.G > kDecRows ? (c * a.G + rows_per_unit - 1) / rows_per_unit : 0;
+        };
+        for (int r = r0; r < r1; r++) {
+            int np, nt, ql;
+            of(r, &np, &nt, &ql);
+            sum += ((unsigned long long)np << 32) | (unsigned)nt;
+            tl += ql;
+        }
+        unsigned long long total;
+        unsigned long long at = block_scan<unsigned long long>(sum, &total, reinterpret_cast<unsigned long long*>(buf));
+        long long ttl, tat = block_scan<long long>(tl, &ttl, buf);
+        for (int r = r0; r < r1; r++) {
+            int np, nt, ql;
+            of(r, &np, &nt, &ql);
+            taken[r] = (int)(at >> 32);
+            touched[r] = (int)(at & 0xffffffffu);
+            tiles[r] = (int)tat;
+            at += ((unsigned long long)np << 32) | (unsigned)nt;
+            tat += ql;
+        }
+        if (threadIdx.x == 0) {
+            taken[n] = (int)(total >> 32);
+            touched[n] = (int)(total & 0xffffffffu);
+            tiles[n] = (int)ttl;
+        }
+    }
+    __syncthreads();
+    uint8_t* work = static_cast<uint8_t*>(s.work);
+
+    if (blockIdx.x > 0) {
+        // ---- rows of the step
+        int4* pages = reinterpret_cast<int4*>(work + a.l.page);
+        const int live = start[n];
+        for (int t = (blockIdx.x - 1) * kRowsPerBlock + threadIdx.x; t < min(s.n_tokens, (int)blockIdx.x * kRowsPerBlock);
+             t += kThreads) {
+            if (t >= live) {
+                s.tok_req[t] = -1;
+                s.tok_pos[t] = 0;
+                s.tok_slot[t] = -1;
+                continue;
+            }
+            const int r = find_last(start, n + 1, t);
+            const int p = past[r], pos = p + t - start[r], j = pos >> lg, off = pos & (ps - 1);
+            const int held = (p + ps - 1) >> lg;
+            int page = -1;
+            if (j < held) {
+                page = __ldg(s.table + (size_t)r * s.max_blocks + j);
+            } else if (j < s.max_blocks) {
+                const int at = nf - 1 - (taken[r] + j - held);
+                if (at >= 0) page = __ldg(a.free_pages + at);
+                if (off == 0) s.table[(size_t)r * s.max_blocks + j] = page;
+            }
+            if (page < 0 || page >= s.n_pages) {
+                err |= SV_DEVERR_PAGES;
+                page = -1;
+            }
+            s.tok_req[t] = r;
+            s.tok_pos[t] = pos;
+            s.tok_slot[t] = page < 0 ? -1 : (page << lg) + off;
+            if (off == 0 || pos == p)
+                pages[touched[r] + j - (p >> lg)] = make_int4(t, page, off, min(ps - off, start[r + 1] - t));
+        }
+    } else {
+        // ---- per request
+        int4* req = reinterpret_cast<int4*>(work + a.l.req);
+        for (int r = threadIdx.x; r < n; r += kThreads) {
+            const int p = past[r], c = start[r + 1] - start[r], held = (p + ps - 1) >> lg;
+            const int got = min(max(nf - taken[r], 0), taken[r + 1] - taken[r]);
+            const int len = (int)min((long long)p + c, ((long long)held + got) << lg);
+            s.q_start[r] = start[r];
+            s.kv_len[r] = len;
+            req[r] = make_int4(start[r], c, p, len);
+        }
+        if (threadIdx.x == 0) {
+            s.q_start[n] = start[n];
+            *a.n_free_out = max(nf - taken[n], 0);
+        }
+        for (int i = threadIdx.x; i < a.l.n_ticks; i += kThreads) reinterpret_cast<int*>(work + a.l.tick)[i] = 0;
+        // ---- decode items: requests of few rows, their keys in splits
+        int2* dec = reinterpret_cast<int2*>(work + a.l.dec);
+        auto dec_cost = [&](int r) {
+            const int c = start[r + 1] - start[r];
+            if (c == 0 || c * a.G > kDecRows) return 0;
+            return (past[r] + c + kDecTile - 1) / kDecTile;
+        };
+        int base = 0;
+        {
+            const int piece = piece_of(n, a.l.dec_slots, kDecMinTiles, dec_cost, buf);
+            for (int u0 = 0; u0 < n; u0 += kThreads) {
+                const int r = u0 + threadIdx.x;
+                const int c = r < n ? dec_cost(r) : 0;
+                const int ns = (c + piece - 1) / piece;
+                long long all, at = block_scan<long long>(ns, &all, buf);
+                for (int i = 0; i < ns; i++) dec[base + at + i] = make_int2(r, i | ns << 16);
+                base += (int)all;
+            }
+        }
+        // ---- prefill items: query tiles of the other requests, last ones (most keys) first
+        int4* pre = reinterpret_cast<int4*>(work + a.l.pre);
+        const int n_tiles = tiles[n], bn = pre_tile(s.head_dim);
+        auto tile_req = [&](int u) { return find_last(tiles, n + 1, u); };
+        auto pre_cost = [&](int u) {
+            const int r = tile_req(u), c = start[r + 1] - start[r];
+            const int last = min(c - 1, ((u - tiles[r] + 1) * rows_per_unit - 1) / a.G);
+            return (past[r] + last + bn) / bn;
+        };
+        int pbase = 0;
+        if (n_tiles > 0) {
+            const int piece = piece_of(n_tiles, a.l.pre_slots, kPreMinTiles, pre_cost, buf);
+            for (int u0 = 0; u0 < n_tiles; u0 += kThreads) {
+                const int u = n_tiles - 1 - (u0 + (int)threadIdx.x);
+                const int ns = u >= 0 ? (pre_cost(u) + piece - 1) / piece : 0;
+                long long all, at = block_scan<long long>(ns, &all, buf);
+                if (u >= 0) {
+                    const int r = tile_req(u);
+                    for (int i = 0; i < ns; i++) pre[pbase + at + i] = make_int4(r, u - tiles[r], i, ns);
+                }
+                pbase += (int)all;
+            }
+        }
+        if (threadIdx.x == 0) {
+            int* head = reinterpret_cast<int*>(work + a.l.head);
+            head[PH_PAGES] = touched[n];
+            head[PH_DEC] = base;
+            head[PH_PRE] = pbase;
+        }
+    }
+    if (err && s.err) atomicOr(s.err, err);
+}
+
+// One block: the pages of the n requests go back in order (exclusive prefix sum of their page counts).
+__global__ void __launch_bounds__(kThreads) paged_release_kernel(int32_t* table, int n_req, int max_blocks, int lg,
+                                                                 int n_pages, const int32_t* req, int n,
+                                                                 const int32_t* kv_len, int32_t* free_pages,
+                                                                 int32_t* n_free, int* err) {
+    __shared__ long long buf[kThreads / 32];
+    pdl_wait();
+    long long at0 = max(__ldg(n_free), 0);
+    int bad = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += kThreads) {
+        const int i = i0 + threadIdx.x;
+        int r = -1, blocks = 0;
+        if (i < n) {
+            r = __ldg(req + i);
+            if (r < 0 || r >= n_req) bad |= SV_DEVERR_STEP;
+            else blocks = (int)min(((long long)max(__ldg(kv_len + i), 0) + (1 << lg) - 1) >> lg, (long long)max_blocks);
+        }
+        long long all, at = at0 + block_scan<long long>(blocks, &all, buf);
+        for (int j = 0; j < blocks; j++, at++) {
+            int32_t* e = table + (size_t)r * max_blocks + j;
+            if (at < n_pages) free_pages[at] = *e;
+            else bad |= SV_DEVERR_PAGES;
+            *e = -1;
+        }
+        at0 += all;
+    }
+    if (threadIdx.x == 0) *n_free = (int)min(at0, (long long)n_pages);
+    if (bad && err) atomicOr(err, bad);
+}
+
+int log2_of(int ps) { return ps == 16 ? 4 : ps == 32 ? 5 : ps == 64 ? 6 : 7; }
+
+}  // namespace
+
+bool step_layout(const sv_paged_step& s, StepLayout* l) {
+    const int ps = s.page_size;
+    if (s.n_req < 1 || s.n_req > SV_PAGED_MAX_REQ || s.n_tokens < 1 || s.max_new < 1 || s.max_blocks < 1 || s.n_pages < 1)
+        return false;
+    if (ps != 16 && ps != 32 && ps != 64 && ps != 128) return false;
+    if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256) return false;
+    if (s.n_kv_head < 1 || s.n_head < 1 || s.n_head % s.n_kv_head != 0) return false;
+    // slots, rows and row x group products stay in 31 bits
+    if ((int64_t)s.n_pages * ps > INT32_MAX || (int64_t)s.max_blocks * ps > INT32_MAX / 2 ||
+        (int64_t)s.n_tokens * s.n_head > INT32_MAX || s.n_kv_head > 1024)
+        return false;
+    const int G = s.n_head / s.n_kv_head, sms = device_sm_count();
+    const int64_t T = s.n_tokens, act = s.n_req < T ? s.n_req : T;
+    const int max_new = s.max_new < T ? s.max_new : (int)T;
+    l->page_cap = (int)(T < T / ps + 2 * act ? T : T / ps + 2 * act);
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    l->dec_slots = (int)up((int64_t)sms * dec_ctas_per_sm(s.head_dim), s.n_kv_head);
+    l->dec_cap = G <= kDecRows ? (int)(act + l->dec_slots) : 0;
+    l->pre_slots = (int)up(sms, s.n_kv_head);
+    const int rows = pre_rows(s.head_dim);
+    if ((int64_t)max_new * G > kDecRows) {
+        const int64_t few = kDecRows / G + 1;    // fewest rows of a prefill request
+        l->pre_cap = (int)(T * G / rows + (act < T / few ? act : T / few) + l->pre_slots);
+    }
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) & ~(size_t)255;
+        return here;
+    };
+    l->n_ticks = (l->dec_cap + l->pre_cap) * s.n_kv_head;
+    l->head = take(128);
+    l->req = take(sizeof(int4) * (size_t)s.n_req);
+    l->page = take(sizeof(int4) * (size_t)l->page_cap);
+    l->dec = take(sizeof(int2) * (size_t)l->dec_cap);
+    l->pre = take(sizeof(int4) * (size_t)l->pre_cap);
+    l->tick = take(sizeof(int) * (size_t)l->n_ticks);
+    l->dec_part = take(sizeof(float) * (size_t)l->dec_cap * s.n_kv_head * kDecRows * s.head_dim);
+    l->dec_ml = take(sizeof(float2) * (size_t)l->dec_cap * s.n_kv_head * kDecRows);
+    l->pre_part = take(sizeof(float) * (size_t)l->pre_cap * s.n_kv_head * rows * s.head_dim);
+    l->pre_ml = take(sizeof(float2) * (size_t)l->pre_cap * s.n_kv_head * rows);
+    l->bytes = at;
+    return true;
+}
+
+cudaError_t launch_paged_plan(const sv_paged_step& s, const StepLayout& l, const int32_t* free_pages,
+                              const int32_t* n_free, int32_t* n_free_out, cudaStream_t st) {
+    PlanArgs a{s, l, free_pages, n_free, n_free_out, s.n_head / s.n_kv_head, log2_of(s.page_size)};
+    const size_t smem = (size_t)(5 * s.n_req + 4) * sizeof(int);
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t status[kMaxDevices];
+    const cudaError_t e = once_per_device(once, status, [] {
+        return cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (5 * SV_PAGED_MAX_REQ + 4) * (int)sizeof(int));
+    });
+    if (e != cudaSuccess) return e;
+    return launch_pdl(paged_plan_kernel, dim3(1 + ceil_div(s.n_tokens, kRowsPerBlock)), dim3(kThreads), smem, st, a);
+}
+
+cudaError_t launch_paged_release(int32_t* table, int n_req, int max_blocks, int ps, int n_pages, const int32_t* req,
+                                 int n, const int32_t* kv_len, int32_t* free_pages, int32_t* n_free, int* err,
+                                 cudaStream_t st) {
+    return launch_pdl(paged_release_kernel, dim3(1), dim3(kThreads), 0, st, table, n_req, max_blocks, log2_of(ps),
+                      n_pages, req, n, kv_len, free_pages, n_free, err);
+}
+
+}  // namespace svkv
