@@ -63,7 +63,7 @@ struct PagedAttn {
     sv_paged kv;
     const int32_t* table;
     int max_blocks;
-    int n_req, n_tokens, n_head, G;
+    int n_req, n_tokens, max_new, n_head, G;
     const uint8_t* q;
     int q_type;
     size_t q_nb;

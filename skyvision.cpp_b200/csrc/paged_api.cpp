@@ -26,7 +26,7 @@ int check_store(const sv_paged* kv) {
     const int ps = kv->page_size, hd = kv->head_dim;
     if (ps != 16 && ps != 32 && ps != 64 && ps != 128) return SV_ERR_UNSUPPORTED;
     if (hd != 64 && hd != 128 && hd != 256) return SV_ERR_UNSUPPORTED;
-    if ((int64_t)kv->n_pages * ps > INT32_MAX || kv->n_kv_head > 1024) return SV_ERR_UNSUPPORTED;
+    if (kv->n_kv_head > 1024 || (int64_t)kv->n_pages * ps * kv->n_kv_head > INT32_MAX) return SV_ERR_UNSUPPORTED;
     return SV_OK;
 }
 
@@ -118,6 +118,7 @@ int sv_paged_attn(const sv_paged* kv, const sv_paged_step* step, const void* q, 
     a.max_blocks = step->max_blocks;
     a.n_req = step->n_req;
     a.n_tokens = step->n_tokens;
+    a.max_new = step->max_new;
     a.n_head = step->n_head;
     a.G = step->n_head / step->n_kv_head;
     a.q = static_cast<const uint8_t*>(q);
@@ -130,7 +131,9 @@ int sv_paged_attn(const sv_paged* kv, const sv_paged_step* step, const void* q, 
     a.work = static_cast<uint8_t*>(step->work);
     a.l = l;
     a.err = kv->err;
-    return status_of(launch_paged_decode(a, static_cast<cudaStream_t>(stream)));
+    cudaError_t e = launch_paged_decode(a, static_cast<cudaStream_t>(stream));
+    if (e == cudaSuccess) e = launch_paged_prefill(a, static_cast<cudaStream_t>(stream));
+    return status_of(e);
 }
 
 }  // extern "C"

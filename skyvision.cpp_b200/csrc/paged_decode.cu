@@ -1,7 +1,30 @@
-// paged_decode.cu - attention over the paged 8-bit cache, one warp per query row and head.
+// paged_decode.cu - attention of requests with few rows over the paged 8-bit cache.
 //
-// o = sum_j p_j v_j / sum_j p_j with p_j = exp2(s_j - m), s_j = scale log2(e) ks[page] (q . c_j), m the running
-// maximum.  Lane l holds elements l + 32 i of q and o.
+// One CTA works on one item of the plan: (request, kv head, a piece of its keys).  The request's rows
+// (new tokens x query heads of the kv head, at most 16) all use every key that is loaded:
+//   s_rj = scale log2(e) ks[page(j)] (q_r . c_j),   p_rj = exp2(s_rj - m_r),
+//   o_r  = sum_j p_rj vs[page(j)] c'_j / sum_j p_rj
+// A scale belongs to a page and head, so it multiplies finished dot products: codes enter the tensor
+// cores as exact f16 integers, and no part of K or V is rounded.
+//
+// A producer warp streams 64-key tiles of codes by TMA (boxes of 16 keys, the smallest page; 128-byte
+// swizzle) into a ring, with each group's two scales; it looks the pages up ahead, 32 groups at a time.
+// Four consumer warps take 16 keys each.  Keys are the M dimension of both products, S^T = C Q^T and
+// O^T += C'^T P^T (m16n8k16), so 8 rows cost one MMA per 16 x 16 codes.  A thread reads 16 bytes of a
+// row at once and spreads them over four k-steps (K) or eight m-tiles (V): the k-order and the m-order
+// of an MMA are free as long as both operands agree, so nothing is transposed in memory.  Bytes become f16
+// by permutes: 0x64uu is 1024 + u, and u = c + 128, so one subtraction of 1152 is exact.
+// The MMA's key index n stands for key n ^ (4 (n & 1)): with the swizzle, the eight lanes of a 16-byte
+// shared load then hit eight different 16-byte columns for K and for V.
+//
+// The running maximum is lazy: a row's reference m_r moves only when a score passes it by 2^8, found by
+// a vote, so a tile normally needs no shuffle and no rescaling; p <= 2^8 is far inside f16.  P is rounded to f16
+// for the second product (2^-12 relative on average, like the f16 output itself); sums stay f32.  P also
+// carries vs / v_ref, where v_ref trails the largest vs seen by at most 4.
+// Pieces of one request and head meet in the work space; the last to arrive (a ticket) adds them in order,
+// so results do not depend on which one that is.
+//
+// Bound: HBM, 2 HD + 8 / page_size bytes per key and kv head.
 #include "common.cuh"
 #include "paged.hpp"
 
@@ -9,71 +32,488 @@ namespace svkv {
 
 namespace {
 
+constexpr int kWarps = 4;                       // consumers
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr float kLazyLog2 = 8.0f;
+
 template <int HD>
-__global__ void __launch_bounds__(256) paged_attn_kernel(const __grid_constant__ PagedAttn a) {
-    constexpr int N = HD / 32;
-    pdl_wait();
-    const int4* req = reinterpret_cast<const int4*>(a.work + a.l.req);
-    const int lane = threadIdx.x & 31;
-    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int t = (int)(id / a.n_head), head = (int)(id % a.n_head), h = head / a.G;
-    if (t >= a.n_tokens) return;
-    int r = 0;
-    for (int lo = 0, hi = a.n_req; hi - lo > 1;) {
-        const int mid = (lo + hi) >> 1;
-        if (req[mid].x <= t) lo = mid;
-        else hi = mid;
-        r = lo;
-    }
-    const int4 q = req[r];
-    if (t >= q.x + q.y) return;
-    const int pos = q.z + t - q.x, end = min(pos + 1, q.w), begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int ps = a.kv.page_size, NKV = a.kv.n_kv_head;
-    float x[N], o[N], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const size_t e = (size_t)head * HD + lane + 32 * i;
-        x[i] = a.q_type == SV_TYPE_F32 ? __half2float(__float2half_rn(reinterpret_cast<const float*>(a.q + (size_t)t * a.q_nb)[e]))
-                                       : __half2float(reinterpret_cast<const __half*>(a.q + (size_t)t * a.q_nb)[e]);
-        o[i] = 0.0f;
-    }
-    for (int j = begin; j < end; j++) {
-        const int page = a.table[(size_t)r * a.max_blocks + j / ps];
-        if (page < 0 || page >= a.kv.n_pages) {
-            if (a.err) atomicOr(a.err, SV_DEVERR_PAGES);
-            continue;
+struct DecCfg {
+    static constexpr int COLS = HD < 128 ? HD : 128;          // bytes of one box row
+    static constexpr int SLABS = HD / COLS;
+    static constexpr int PART = kDecTile * HD;                // K or V codes of a tile
+    static constexpr int STAGE = 2 * PART;
+    static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 4 : 3;
+    static constexpr int OFF_SC = STAGES * STAGE;             // float2 [STAGES][4]: K and V scale of each group
+    static constexpr int OFF_OK = OFF_SC + STAGES * 32;       // int [STAGES][4]: the group's page exists
+    static constexpr int OFF_BAR = OFF_OK + STAGES * 16;
+    static constexpr int OFF_ML = OFF_BAR + STAGES * 16;      // float [3][kWarps][16]
+    static constexpr int SMEM = OFF_ML + 3 * kWarps * 16 * 4 + 16;
+    static constexpr int PITCH = HD + 4;                      // floats per row of the warps' partial outputs
+    static_assert(kWarps * kDecRows * PITCH * 4 <= OFF_SC, "the warps' partials reuse the ring");
+};
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+
+// two biased codes (c + 128) in the low or high half of w -> f16 c
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+    const uint32_t h = prmt(w, 0x64646464u, 0x4140);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+    const uint32_t h = prmt(w, 0x64646464u, 0x4342);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t movm_t(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// byte offset of 16-byte column c of row r in a box of COLS-byte rows (128- or 64-byte swizzle)
+template <int COLS>
+__device__ __forceinline__ uint32_t col16(uint32_t r, uint32_t c) {
+    return COLS == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// NT: row tiles of 8
+template <int HD, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? dec_ctas_per_sm(HD) : dec_ctas_per_sm(HD) - 1)
+paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                    const __grid_constant__ PagedAttn a) {
+    using C = DecCfg<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float2* sc = reinterpret_cast<float2*>(smem + C::OFF_SC);
+    int* okp = reinterpret_cast<int*>(smem + C::OFF_OK);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* empty = full + C::STAGES;
+    float* s_ml = reinterpret_cast<float*>(smem + C::OFF_ML);
+    int* s_last = reinterpret_cast<int*>(s_ml + 3 * kWarps * 16);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int NKV = a.kv.n_kv_head;
+    const int h = blockIdx.x % NKV, item = blockIdx.x / NKV;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], kWarps);
         }
-        const size_t unit = (size_t)page * NKV + h, off = (unit * ps + j % ps) * HD;
-        const int8_t* k = static_cast<const int8_t*>(a.kv.k) + off;
-        const int8_t* v = static_cast<const int8_t*>(a.kv.v) + off;
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; i++) s = fmaf(x[i], (float)k[lane + 32 * i], s);
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        s *= a.kv.k_scale[unit] * a.scale_log2;
-        const float mn = fmaxf(m, s), f = exp2f(m - mn), p = exp2f(s - mn), pv = p * a.kv.v_scale[unit];
-        l = l * f + p;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = fmaf(pv, (float)v[lane + 32 * i], o[i] * f);
+        fence_barrier_init();
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const size_t e = ((size_t)t * a.n_head + head) * HD + lane + 32 * i;
-        if (a.out_type == SV_TYPE_F32) static_cast<float*>(a.out)[e] = o[i] * inv;
-        else static_cast<__half*>(a.out)[e] = __float2half_rn(o[i] * inv);
+    if (threadIdx.x == 32) {
+        tma_prefetch_desc(&tmk);
+        tma_prefetch_desc(&tmv);
     }
+    __syncthreads();
+    pdl_wait();
+    if (threadIdx.x == 0) pdl_trigger();
+    const int n_items = reinterpret_cast<const int*>(a.work + a.l.head)[PH_DEC];
+    if (item >= n_items) return;
+    const int2 it = reinterpret_cast<const int2*>(a.work + a.l.dec)[item];
+    const int split = it.y & 0xffff, ns = it.y >> 16;
+    const int4 rq = reinterpret_cast<const int4*>(a.work + a.l.req)[it.x];   // first row, rows, held before, after
+    const int rows = rq.y * a.G;
+    if ((rows > 8) != (NT == 2)) return;
+    const int lo_key = a.window > 0 ? max(0, rq.z - a.window + 1) : 0;
+    const int t_lo = lo_key / kDecTile, t_hi = (rq.w + kDecTile - 1) / kDecTile;
+    const int nt_all = max(0, t_hi - t_lo);
+    const int j0 = t_lo + (int)((long long)nt_all * split / ns), j1 = t_lo + (int)((long long)nt_all * (split + 1) / ns);
+    const int n = j1 - j0;
+
+    if (warp == kWarps) {
+        // ================= producer: lane g holds group j0 * 4 + (batch of 32) + g's page and scales
+        const int lg = 31 - __clz(a.kv.page_size);
+        const int g_end = (rq.w + 15) >> 4;                       // groups that hold a key
+        const int32_t* row = a.table + (size_t)it.x * a.max_blocks;
+        auto page_of = [&](int g) { return g < min(g_end, 4 * j1) ? __ldg(row + ((g << 4) >> lg)) : 0; };
+        auto valid = [&](int g, int p) { return g < g_end && p >= 0 && p < a.kv.n_pages; };
+        int p0 = page_of(4 * j0 + lane);
+        int p1 = page_of(4 * j0 + 32 + lane);
+        float2 s0 = make_float2(0.0f, 0.0f);
+        bool v0 = valid(4 * j0 + lane, p0);
+        auto scales = [&](int p, bool v) {
+            float2 s = make_float2(0.0f, 0.0f);
+            if (v) {
+                s.x = __ldg(a.kv.k_scale + (size_t)p * NKV + h);
+                s.y = __ldg(a.kv.v_scale + (size_t)p * NKV + h);
+            }
+            return s;
+        };
+        s0 = scales(p0, v0);
+        float2 s1 = scales(p1, valid(4 * j0 + 32 + lane, p1));
+        for (int i = 0; i < n; i++) {
+            const int st = i % C::STAGES, at = (4 * i) & 31;
+            if (i > 0 && at == 0) {                               // the next 32 groups, looked up 8 tiles ago
+                p0 = p1;
+                s0 = s1;
+                const int g = 4 * (j0 + i) + 32 + lane;
+                v0 = valid(g - 32, p0);
+                p1 = page_of(g);
+                s1 = scales(p1, valid(g, p1));
+            }
+            bool ok = true;
+            if (lane == 0 && i >= C::STAGES) ok = mbar_wait(&empty[st], ((i / C::STAGES) + 1) & 1, a.err);
+            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+            const int src = at + (lane & 3);
+            const int page = __shfl_sync(0xffffffffu, p0, src);
+            const bool v = __shfl_sync(0xffffffffu, (int)v0, src) != 0;
+            const float2 s = make_float2(__shfl_sync(0xffffffffu, s0.x, src), __shfl_sync(0xffffffffu, s0.y, src));
+            const int grp = 4 * (j0 + i) + (lane & 3);
+            if (lane < 4) {
+                sc[st * 4 + lane] = make_float2(s.x * a.scale_log2, s.y);
+                okp[st * 4 + lane] = v;
+                if (!v && grp < g_end && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
+            }
+            const unsigned have = __ballot_sync(0xffffffffu, v && lane < 4);
+            if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * 16 * HD * 2));
+            __syncwarp();
+            if (v && lane < 8 * C::SLABS) {
+                const bool is_v = (lane & 4) != 0;
+                const int slab = lane >> 3;
+                const int y = ((page * NKV + h) << lg) + ((grp << 4) & (a.kv.page_size - 1));
+                uint8_t* dst = smem + st * C::STAGE + (is_v ? C::PART : 0) + slab * (kDecTile * C::COLS) + (lane & 3) * 16 * C::COLS;
+                tma_load_2d(dst, is_v ? &tmv : &tmk, slab * C::COLS, y, &full[st]);
+            }
+        }
+        // the ring becomes the warps' scratch below: every load has landed, since every tile was waited for
+    } else {
+        // ================= consumers
+        const int gq = lane >> 2, tq = lane & 3;
+        // Q^T fragments: row gq (of each row tile), bytes 16 tq.. of each 64-dim group over four k-steps
+        uint32_t qf[NT][HD / 64][8];
+#pragma unroll
+        for (int r = 0; r < NT; r++) {
+            const int rr = r * 8 + gq;
+            const bool live = rr < rows;
+            const uint8_t* qp = a.q + (size_t)(rq.x + (live ? rr / a.G : 0)) * a.q_nb;
+            const int col = (h * a.G + (live ? rr % a.G : 0)) * HD + 16 * tq;
+#pragma unroll
+            for (int g = 0; g < HD / 64; g++) {
+                if (a.q_type == SV_TYPE_F32) {
+                    const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qp) + col + 64 * g);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4 x = live ? f[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        qf[r][g][2 * i] = pack_h2(x.x, x.y);
+                        qf[r][g][2 * i + 1] = pack_h2(x.z, x.w);
+                    }
+                } else {
+                    const uint4* f = reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(qp) + col + 64 * g);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const uint4 x = live ? f[i] : make_uint4(0, 0, 0, 0);
+                        qf[r][g][4 * i] = x.x;
+                        qf[r][g][4 * i + 1] = x.y;
+                        qf[r][g][4 * i + 2] = x.z;
+                        qf[r][g][4 * i + 3] = x.w;
+                    }
+                }
+            }
+        }
+        // this thread's columns: rows 8 r + 2 tq + {0, 1}; keys they see: [lo, hi)
+        int lo[NT][2], hi[NT][2];
+        int lo_max = 0, hi_min = INT32_MAX;
+#pragma unroll
+        for (int r = 0; r < NT; r++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int pos = rq.z + min(8 * r + 2 * tq + e, rows - 1) / a.G;
+                lo[r][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+                hi[r][e] = min(pos + 1, rq.w);
+                lo_max = max(lo_max, lo[r][e]);
+                hi_min = min(hi_min, hi[r][e]);
+            }
+        float o[HD / 16][NT][4];
+#pragma unroll
+        for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+            for (int r = 0; r < NT; r++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[m][r][e] = 0.0f;
+        float mref[NT][2], l[NT][2], vref = 0.0f, vinv = 0.0f;
+#pragma unroll
+        for (int r = 0; r < NT; r++) mref[r][0] = mref[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
+        const int k0 = gq & 1 ? gq ^ 4 : gq;                       // key of MMA index gq
+        const int c0 = 2 * tq, c1 = (2 * tq + 1) ^ 4;              // keys of MMA indexes 2 tq, 2 tq + 1
+
+        for (int i = 0; i < n; i++) {
+            const int st = i % C::STAGES;
+            const bool got = mbar_wait(&full[st], (i / C::STAGES) & 1, a.err);
+            if (!__all_sync(0xffffffffu, got)) break;
+            const int kb = (j0 + i) * kDecTile + 16 * warp;        // first key of this warp's group
+            const float2 s2 = sc[st * 4 + warp];
+            const bool there = okp[st * 4 + warp] != 0;
+            if (there && kb < rq.w) {
+                const uint8_t* kt = smem + st * C::STAGE;
+                const uint8_t* vt = kt + C::PART;
+                float s[NT][4];
+#pragma unroll
+                for (int r = 0; r < NT; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[r][e] = 0.0f;
+#pragma unroll
+                for (int g = 0; g < HD / 64; g++) {
+                    const int slab = g * 64 / C::COLS, cc = (g * 64 % C::COLS) / 16 + tq;
+                    const uint8_t* base = kt + slab * (kDecTile * C::COLS);
+                    const uint4 wa = *reinterpret_cast<const uint4*>(base + col16<C::COLS>(16 * warp + k0, cc));
+                    const uint4 wb = *reinterpret_cast<const uint4*>(base + col16<C::COLS>(16 * warp + 8 + k0, cc));
+                    const uint32_t xa[4] = {wa.x, wa.y, wa.z, wa.w}, xb[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t ua = xa[j] ^ 0x80808080u, ub = xb[j] ^ 0x80808080u;
+                        const uint32_t f[4] = {codes_lo(ua), codes_lo(ub), codes_hi(ua), codes_hi(ub)};
+#pragma unroll
+                        for (int r = 0; r < NT; r++) mma_f16(s[r], f, qf[r][g][2 * j], qf[r][g][2 * j + 1]);
+                    }
+                }
+                // scores of keys k0 (s[r][0..1]) and 8 + k0 (s[r][2..3]), rows 2 tq + {0, 1}
+                bool over = false;
+#pragma unroll
+                for (int r = 0; r < NT; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[r][e] *= s2.x;
+                if (kb < lo_max || kb + 16 > hi_min) {
+#pragma unroll
+                    for (int r = 0; r < NT; r++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int key = kb + k0 + (e >> 1) * 8;
+                            if (key < lo[r][e & 1] || key >= hi[r][e & 1]) s[r][e] = -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int r = 0; r < NT; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) over |= s[r][e] > mref[r][e & 1] + kLazyLog2;
+                if (__any_sync(0xffffffffu, over || s2.y > 4.0f * vref)) {
+                    float vf = 1.0f;
+                    if (s2.y > vref) {
+                        vf = vref / s2.y;
+                        vref = s2.y;
+                        vinv = 1.0f / vref;
+                    }
+#pragma unroll
+                    for (int r = 0; r < NT; r++) {
+                        float f[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float mx = fmaxf(s[r][e], s[r][e + 2]);
+#pragma unroll
+                            for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+                            const float mn = fmaxf(mref[r][e], mx);
+                            const float g = mn == -INFINITY ? 1.0f : fast_exp2(mref[r][e] - mn);
+                            l[r][e] *= g;
+                            mref[r][e] = mn;
+                            f[e] = g * vf;
+                        }
+#pragma unroll
+                        for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[m][r][e] *= f[e & 1];
+                    }
+                }
+                const float pv = s2.y * vinv;
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int r = 0; r < NT; r++) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float m = mref[r][e & 1];
+                        p[e] = fast_exp2(s[r][e] - (m == -INFINITY ? 0.0f : m));
+                    }
+                    l[r][0] += p[0] + p[2];
+                    l[r][1] += p[1] + p[3];
+                    pb[r][0] = movm_t(pack_h2(p[0] * pv, p[1] * pv));
+                    pb[r][1] = movm_t(pack_h2(p[2] * pv, p[3] * pv));
+                }
+                // V: 16 bytes (8 at HD 64) of keys c0, c1, 8 + c0, 8 + c1
+                constexpr int VB = HD >= 128 ? 16 : 8;
+#pragma unroll
+                for (int slab = 0; slab < C::SLABS; slab++) {
+                    uint32_t w[4][VB / 4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int key = 16 * warp + (k & 1 ? c1 : c0) + (k >> 1) * 8;
+                        const uint8_t* base = vt + slab * (kDecTile * C::COLS);
+                        if constexpr (VB == 16) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(base + col16<C::COLS>(key, gq));
+                            w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
+                        } else {
+                            const uint2 x = *reinterpret_cast<const uint2*>(base + col16<C::COLS>(key, gq >> 1) + (gq & 1) * 8);
+                            w[k][0] = x.x; w[k][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < VB / 4; j++) {
+                        const uint32_t u0 = w[0][j] ^ 0x80808080u, u1 = w[1][j] ^ 0x80808080u;
+                        const uint32_t u2 = w[2][j] ^ 0x80808080u, u3 = w[3][j] ^ 0x80808080u;
+#pragma unroll
+                        for (int d = 0; d < 2; d++) {              // dims 4 j + 2 d + {0, 1} of this thread's run
+                            const uint32_t x = prmt(u0, u1, d ? 0x7362 : 0x5140), y = prmt(u2, u3, d ? 0x7362 : 0x5140);
+                            const uint32_t f[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
+#pragma unroll
+                            for (int r = 0; r < NT; r++)
+                                mma_f16(o[slab * (VB / 2) + 2 * j + d][r], f, pb[r][0], pb[r][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+        // ---- this warp's partial: row sums over the quads' lanes, outputs in v_ref units
+#pragma unroll
+        for (int r = 0; r < NT; r++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], w);
+        asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");   // every consumer is past the ring
+        float* part = reinterpret_cast<float*>(smem) + warp * kDecRows * C::PITCH;
+        constexpr int VB = HD >= 128 ? 16 : 8;
+#pragma unroll
+        for (int m = 0; m < HD / 16; m++) {
+            const int d = (m / (VB / 2)) * 128 + VB * gq + 2 * (m % (VB / 2));
+#pragma unroll
+            for (int r = 0; r < NT; r++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    *reinterpret_cast<float2*>(part + (8 * r + 2 * tq + e) * C::PITCH + d) =
+                        make_float2(o[m][r][e] * vref, o[m][r][e + 2] * vref);
+        }
+        if (gq == 0) {
+#pragma unroll
+            for (int r = 0; r < NT; r++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    s_ml[warp * 16 + 8 * r + 2 * tq + e] = mref[r][e];
+                    s_ml[(kWarps + warp) * 16 + 8 * r + 2 * tq + e] = l[r][e];
+                }
+        }
+    }
+    __syncthreads();
+    // ---- the warps' partials of each row become one
+    const int unit = item * NKV + h, first = (item - split) * NKV + h;
+    float* wo = reinterpret_cast<float*>(a.work + a.l.dec_part) + (size_t)unit * kDecRows * HD;
+    float2* wml = reinterpret_cast<float2*>(a.work + a.l.dec_ml) + (size_t)unit * kDecRows;
+    auto store = [&](int r, int d, float4 x) {
+        const size_t at = ((size_t)(rq.x + r / a.G) * a.n_head + h * a.G + r % a.G) * HD + d;
+        if (a.out_type == SV_TYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = x;
+        else *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at) = make_uint2(pack_h2(x.x, x.y), pack_h2(x.z, x.w));
+    };
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w * 16 + r]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float m = s_ml[w * 16 + r], f = m == -INFINITY ? 0.0f : fast_exp2(m - M);
+            const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + (w * kDecRows + r) * C::PITCH + d);
+            L = fmaf(f, s_ml[(kWarps + w) * 16 + r], L);
+            x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+        }
+        if (ns == 1) {
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+            store(r, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        } else {
+            *reinterpret_cast<float4*>(wo + (size_t)r * HD + d) = x;
+            if (d == 0) wml[r] = make_float2(M, L);
+        }
+    }
+    if (ns == 1) return;
+    // ---- pieces of one request and head: the last to arrive adds them, in order
+    __threadfence();
+    __syncthreads();
+    int* ticket = reinterpret_cast<int*>(a.work + a.l.tick) + first;
+    if (threadIdx.x == 0) {
+        const int last = atomicAdd(ticket, 1) == ns - 1;
+        if (last) *ticket = 0;                                     // ready for the next layer
+        *s_last = last;
+    }
+    __syncthreads();
+    if (!*s_last) return;
+    __threadfence();
+    const float* po = reinterpret_cast<const float*>(a.work + a.l.dec_part) + (size_t)first * kDecRows * HD;
+    const float2* pml = reinterpret_cast<const float2*>(a.work + a.l.dec_ml) + (size_t)first * kDecRows;
+    const size_t so = (size_t)NKV * kDecRows * HD, sm = (size_t)NKV * kDecRows;
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        float M = -INFINITY, L = 0.0f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < ns; s0 += 8) {                       // eight pieces' loads in flight
+            float2 ml[8];
+            float4 y[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const int s = min(s0 + u, ns - 1);
+                ml[u] = __ldcg(pml + s * sm + r);
+                y[u] = __ldcg(reinterpret_cast<const float4*>(po + s * so + (size_t)r * HD + d));
+            }
+            float mn = M;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                if (s0 + u >= ns) ml[u] = make_float2(-INFINITY, 0.0f);
+                mn = fmaxf(mn, ml[u].x);
+            }
+            if (mn == -INFINITY) continue;
+            const float g = M == -INFINITY ? 0.0f : fast_exp2(M - mn);
+            M = mn;
+            L *= g;
+            x.x *= g; x.y *= g; x.z *= g; x.w *= g;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float f = ml[u].x == -INFINITY ? 0.0f : fast_exp2(ml[u].x - mn);
+                L = fmaf(f, ml[u].y, L);
+                x.x = fmaf(f, y[u].x, x.x); x.y = fmaf(f, y[u].y, x.y); x.z = fmaf(f, y[u].z, x.z); x.w = fmaf(f, y[u].w, x.w);
+            }
+        }
+        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+        store(r, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    }
+}
+
+template <int HD>
+cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
+    using C = DecCfg<HD>;
+    constexpr int smem = C::SMEM + 1024;
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t status[kMaxDevices];
+    const cudaError_t e = once_per_device(once, status, [] {
+        const cudaError_t x = cudaFuncSetAttribute(paged_decode_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return x != cudaSuccess ? x : cudaFuncSetAttribute(paged_decode_kernel<HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    });
+    if (e != cudaSuccess) return e;
+    CUtensorMap tmk, tmv;
+    const uint64_t rows = (uint64_t)a.kv.n_pages * a.kv.n_kv_head * a.kv.page_size;
+    const CUtensorMapSwizzle swz = C::COLS == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    if (!encode_tmap_2d(&tmk, a.kv.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz) ||
+        !encode_tmap_2d(&tmv, a.kv.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz))
+        return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)(a.l.dec_cap * a.kv.n_kv_head));
+    // Requests of up to 8 rows and of 9 to 16 take different kernels; either launch is left out where the
+    // step's bounds rule its requests out.
+    cudaError_t rc = cudaSuccess;
+    if (a.G <= 8) rc = launch_pdl(paged_decode_kernel<HD, 1>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
+    if (rc == cudaSuccess && (int64_t)a.max_new * a.G > 8)
+        rc = launch_pdl(paged_decode_kernel<HD, 2>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
+    return rc;
 }
 
 }  // namespace
 
 cudaError_t launch_paged_decode(const PagedAttn& a, cudaStream_t st) {
-    const dim3 grid((unsigned)(((int64_t)a.n_tokens * a.n_head + 7) / 8));
-    if (a.kv.head_dim == 64) return launch_pdl(paged_attn_kernel<64>, grid, dim3(256), 0, st, a);
-    if (a.kv.head_dim == 128) return launch_pdl(paged_attn_kernel<128>, grid, dim3(256), 0, st, a);
-    return launch_pdl(paged_attn_kernel<256>, grid, dim3(256), 0, st, a);
+    if (a.l.dec_cap == 0) return cudaSuccess;
+    switch (a.kv.head_dim) {
+        case 64: return launch_hd<64>(a, st);
+        case 128: return launch_hd<128>(a, st);
+        default: return launch_hd<256>(a, st);
+    }
 }
 
 }  // namespace svkv

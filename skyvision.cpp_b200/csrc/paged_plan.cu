@@ -303,9 +303,9 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     if (ps != 16 && ps != 32 && ps != 64 && ps != 128) return false;
     if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256) return false;
     if (s.n_kv_head < 1 || s.n_head < 1 || s.n_head % s.n_kv_head != 0) return false;
-    // slots, rows and row x group products stay in 31 bits
-    if ((int64_t)s.n_pages * ps > INT32_MAX || (int64_t)s.max_blocks * ps > INT32_MAX / 2 ||
-        (int64_t)s.n_tokens * s.n_head > INT32_MAX || s.n_kv_head > 1024)
+    // rows of the pool, positions and row x head products stay in 31 bits
+    if (s.n_kv_head > 1024 || (int64_t)s.n_pages * ps * s.n_kv_head > INT32_MAX || (int64_t)s.max_blocks * ps > INT32_MAX / 2 ||
+        (int64_t)s.n_tokens * s.n_head > INT32_MAX)
         return false;
     const int G = s.n_head / s.n_kv_head, sms = device_sm_count();
     const int64_t T = s.n_tokens, act = s.n_req < T ? s.n_req : T;
