@@ -1,80 +1,568 @@
-// paged_prefill.cu - attention of requests with many rows over the paged 8-bit cache, one warp per query row and head.
+// paged_prefill.cu - attention of requests with many rows over the paged 8-bit cache: tcgen05.mma with the
+// accumulators in TMEM.
 //
-// o = sum_j p_j v_j / sum_j p_j with p_j = exp2(s_j - m), s_j = scale log2(e) ks[page] (q . c_j), m the running
-// maximum.  Lane l holds elements l + 32 i of q and o.
+//   s_rj = scale log2(e) ks[page(j)] (q_r . c_j),   p_rj = exp2(s_rj - m_r),
+//   o_r  = sum_j p_rj vs[page(j)] c'_j / sum_j p_rj
+// The scales belong to a page and head, so both products run on the codes alone, which are exact in f16: one MMA
+// part per tile where a block-scaled row format needs two.  ks is applied to finished scores, vs / v_ref to the
+// weights before they are rounded to f16 (2^-12 relative on average, like an f16 output); sums stay f32.
+//
+// Work item (from the plan): NQT tiles of 128 rows of one request and kv head (rows = tokens x the G query
+// heads, packed, so any G fills them) x a piece of the keys they see.  Roles:
+//   softmax warps   4 per row tile, one row per thread: S from TMEM, scales, causal / window mask, maximum, P as
+//                   f16 back over the S columns.  m_r is lazy: it moves (and O is rescaled in TMEM) only when
+//                   a row of the warp passes it by 2^8, so most tiles never touch O.
+//   converter warps read code tiles (16 bytes a thread, straight from the pages), turn bytes into f16 by
+//                   permutes (0x64uu = 1024 + u; minus 1152 is exact) and write them 128-byte swizzled into
+//                   a ring of K and V tiles; the loads of the next tile are issued as each piece is stored.
+//   MMA thread      S = Q K^T (both K-major), O += P V (P from TMEM, V MN-major).
+// With two row tiles (HD 64, 128; 128 keys) each has one S buffer and they alternate on the tensor core; with
+// one (HD 256; 64 keys) S is double-buffered.
+// Pieces of an item's rows meet in the work space; the last to arrive adds them in order.
+//
+// Bound: tensor pipe and exponentials (4 NH HD flops and NH exponentials per visible pair).
 #include "common.cuh"
 #include "paged.hpp"
+#include "umma.cuh"
 
 namespace svkv {
 
 namespace {
 
+constexpr float kLazyLog2 = 8.0f;
+
 template <int HD>
-__global__ void __launch_bounds__(256) paged_attn_kernel(const __grid_constant__ PagedAttn a) {
-    constexpr int N = HD / 32;
+struct PreCfgP {
+    static constexpr int NQT = HD == 256 ? 1 : 2;
+    static constexpr int BN = pre_tile(HD);
+    static constexpr bool S2 = NQT == 1;                  // S double-buffered
+    static constexpr int ROWS = NQT * 128;
+    static constexpr int QBOX = 128 * 128;                // one 64-column slab of a row tile
+    static constexpr int Q_B = (HD / 64) * QBOX;
+    static constexpr int KBOX = BN * 128;                 // one 64-column slab of a K or V tile
+    static constexpr int KV_B = (HD / 64) * KBOX;
+    static constexpr int FIT = (227 * 1024 - 6144 - NQT * Q_B) / KV_B;
+    static constexpr int NE = FIT > 8 ? 8 : FIT;          // ring entries: K0 V0 K1 V1 ...
+    static constexpr int SM_WARPS = 4 * NQT;
+    static constexpr int CV_WARPS = 4;
+    // Two row tiles: four warpgroups of 128 registers a thread at launch, split again by need
+    // (256 x 192 + 128 x 80 + 128 x 48 = 512 x 128).  One row tile fits as it is.
+    static constexpr bool SPLIT_REGS = NQT == 2;
+    static constexpr int THREADS = SPLIT_REGS ? 512 : (SM_WARPS + CV_WARPS + 1) * 32;
+    static constexpr int GROUPS = BN / 16;                // 16-key groups of a tile
+    static constexpr int OFF_RING = NQT * Q_B;
+    static constexpr int OFF_SC = OFF_RING + NE * KV_B;   // float2 [SM_WARPS][2][32]
+    static constexpr int OFF_BAR = OFF_SC + SM_WARPS * 2 * 32 * 8;
+    static constexpr int N_BAR = 2 * NE + 1 + NQT * 6;
+    static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 32;
+    static_assert(SMEM + 1024 <= 227 * 1024, "shared memory budget");
+    static constexpr int SCOLS = 128;                     // S/P columns per row tile, O after them
+    static constexpr int QCOLS = SCOLS + HD;
+    static constexpr int TMEM_COLS = 512;
+    static_assert(NQT * QCOLS <= 512, "TMEM budget");
+};
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                            uint32_t acc) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        ".reg .b64 db;\n"
+        "setp.ne.b32 p, %5, 0;\n"
+        "mov.b64 db, {%2, %3};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n"
+        "}\n" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc));
+}
+
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t sel) {
+    const uint32_t h = __byte_perm(w, 0x64646464u, sel);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// two f32 lanes in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+          "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int HD>
+__global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ PagedAttn a) {
+    using C = PreCfgP<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t* full = bars;                      // [NE] converters -> MMA
+    uint64_t* empty = bars + C::NE;             // [NE] MMA -> converters
+    uint64_t* q_full = bars + 2 * C::NE;
+    uint64_t* s_full = q_full + 1;              // [NQT][2]
+    uint64_t* p_full = s_full + 2 * C::NQT;     // [NQT][2]
+    uint64_t* o_done = p_full + 2 * C::NQT;     // [NQT][2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::N_BAR);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* s_last = abort_flag + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int NKV = a.kv.n_kv_head;
+    const int h = blockIdx.x % NKV, item = blockIdx.x / NKV;
     pdl_wait();
-    const int4* req = reinterpret_cast<const int4*>(a.work + a.l.req);
-    const int lane = threadIdx.x & 31;
-    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int t = (int)(id / a.n_head), head = (int)(id % a.n_head), h = head / a.G;
-    if (t >= a.n_tokens) return;
-    int r = 0;
-    for (int lo = 0, hi = a.n_req; hi - lo > 1;) {
-        const int mid = (lo + hi) >> 1;
-        if (req[mid].x <= t) lo = mid;
-        else hi = mid;
-        r = lo;
-    }
-    const int4 q = req[r];
-    if (t >= q.x + q.y || q.y * a.G <= kDecRows) return;
-    const int pos = q.z + t - q.x, end = min(pos + 1, q.w), begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const int ps = a.kv.page_size, NKV = a.kv.n_kv_head;
-    float x[N], o[N], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const size_t e = (size_t)head * HD + lane + 32 * i;
-        x[i] = a.q_type == SV_TYPE_F32 ? __half2float(__float2half_rn(reinterpret_cast<const float*>(a.q + (size_t)t * a.q_nb)[e]))
-                                       : __half2float(reinterpret_cast<const __half*>(a.q + (size_t)t * a.q_nb)[e]);
-        o[i] = 0.0f;
-    }
-    for (int j = begin; j < end; j++) {
-        const int page = a.table[(size_t)r * a.max_blocks + j / ps];
-        if (page < 0 || page >= a.kv.n_pages) {
-            if (a.err) atomicOr(a.err, SV_DEVERR_PAGES);
-            continue;
+    if (threadIdx.x == 0) pdl_trigger();
+    if (item >= reinterpret_cast<const int*>(a.work + a.l.head)[PH_PRE]) return;
+    const int4 it = reinterpret_cast<const int4*>(a.work + a.l.pre)[item];         // request, row tile, split, splits
+    const int4 rq = reinterpret_cast<const int4*>(a.work + a.l.req)[it.x];         // first row, rows, held before, after
+    const int split = it.z, ns = it.w;
+    const int row0 = it.y * C::ROWS;
+    const int n_rows = min(C::ROWS, rq.y * a.G - row0);
+    const int nqt = (n_rows + 127) / 128;
+    const int tok0 = row0 / a.G, tok1 = (row0 + n_rows - 1) / a.G;
+    const int lo_key = a.window > 0 ? max(0, rq.z + tok0 - a.window + 1) : 0;
+    const int hi_key = min(rq.z + tok1 + 1, rq.w);
+    const int t_lo = lo_key / C::BN, t_hi = (hi_key + C::BN - 1) / C::BN;
+    const int nt_all = max(0, t_hi - t_lo);
+    const int j0 = t_lo + (int)((long long)nt_all * split / ns), j1 = t_lo + (int)((long long)nt_all * (split + 1) / ns);
+    const int n = j1 - j0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::NE; s++) {
+            mbar_init(&full[s], C::CV_WARPS);
+            mbar_init(&empty[s], 1);
         }
-        const size_t unit = (size_t)page * NKV + h, off = (unit * ps + j % ps) * HD;
-        const int8_t* k = static_cast<const int8_t*>(a.kv.k) + off;
-        const int8_t* v = static_cast<const int8_t*>(a.kv.v) + off;
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; i++) s = fmaf(x[i], (float)k[lane + 32 * i], s);
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-        s *= a.kv.k_scale[unit] * a.scale_log2;
-        const float mn = fmaxf(m, s), f = exp2f(m - mn), p = exp2f(s - mn), pv = p * a.kv.v_scale[unit];
-        l = l * f + p;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < N; i++) o[i] = fmaf(pv, (float)v[lane + 32 * i], o[i] * f);
+        mbar_init(q_full, 4 * C::NQT);
+        for (int i = 0; i < 2 * C::NQT; i++) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const size_t e = ((size_t)t * a.n_head + head) * HD + lane + 32 * i;
-        if (a.out_type == SV_TYPE_F32) static_cast<float*>(a.out)[e] = o[i] * inv;
-        else static_cast<__half*>(a.out)[e] = __float2half_rn(o[i] * inv);
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"((uint32_t)C::TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int lg = 31 - __clz(a.kv.page_size);
+    const int g_end = (rq.w + 15) >> 4;                    // 16-key groups that hold a key
+    const int32_t* trow = a.table + (size_t)it.x * a.max_blocks;
+    const int g_stop = min(g_end, j1 * C::GROUPS);
+    auto page_of = [&](int g) { return g < g_stop ? __ldg(trow + ((g << 4) >> lg)) : -1; };
+    auto valid = [&](int p) { return p >= 0 && p < a.kv.n_pages; };
+
+    if (warp < C::SM_WARPS) {
+        // ============================ softmax: one row per thread
+        if constexpr (C::SPLIT_REGS) regs_up<192>();
+        const int qtl = warp >> 2, quarter = warp & 3;
+        const bool tile_live = qtl < nqt;
+        const int r = quarter * 32 + lane, flat = qtl * 128 + r;
+        const bool live = flat < n_rows;
+        const int rr = row0 + (live ? flat : n_rows - 1);
+        const int tok = rr / a.G, hd = h * a.G + rr % a.G;
+        const int pos = rq.z + tok;
+        const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, hi = min(pos + 1, rq.w);
+        const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(qtl * C::QCOLS);
+        {
+            const uint8_t* qrow = a.q + (size_t)(rq.x + tok) * a.q_nb;
+            uint8_t* qs = smem + qtl * C::Q_B;
+#pragma unroll 4
+            for (int e = 0; e < HD; e += 8) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (live) {
+                    if (a.q_type == SV_TYPE_F32) {
+                        const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qrow) + (size_t)hd * HD + e);
+                        const float4 f0 = f[0], f1 = f[1];
+                        v = make_uint4(pack_h2(f0.x, f0.y), pack_h2(f0.z, f0.w), pack_h2(f1.x, f1.y), pack_h2(f1.z, f1.w));
+                    } else {
+                        v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(qrow) + (size_t)hd * HD + e);
+                    }
+                }
+                *reinterpret_cast<uint4*>(qs + (e / 64) * C::QBOX + swz_off(r, e % 64, 128)) = v;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        // Scales of 32 groups at a time in this warp's own table: x = ks scale log2(e) (a page of zeros has
+        // zero scores at any x > 0), y = vs; a group without a page has x < 0.
+        float2* sc = reinterpret_cast<float2*>(smem + C::OFF_SC) + warp * 64;
+        constexpr int TPB = 32 / C::GROUPS;                 // tiles per batch of 32 groups
+        auto scale_of = [&](int g, int p) {
+            float2 s = make_float2(-1.0f, 0.0f);
+            if (g < g_stop && valid(p)) {
+                s.x = fmaxf(__ldg(a.kv.k_scale + (size_t)p * NKV + h) * a.scale_log2, 1.17549435e-38f);
+                s.y = __ldg(a.kv.v_scale + (size_t)p * NKV + h);
+            }
+            return s;
+        };
+        int pg = page_of(j0 * C::GROUPS + lane);
+        float2 next = scale_of(j0 * C::GROUPS + lane, pg);
+        pg = page_of(j0 * C::GROUPS + 32 + lane);
+        float m = -INFINITY, vref = 0.0f;
+        float2 l2 = make_float2(0.0f, 0.0f);
+        bool ok = true;
+        const int n_mine = tile_live ? n : 0;
+        for (int i = 0; i < n_mine; i++) {
+            const int at = (i % TPB) * C::GROUPS;
+            float2* tab = sc + ((i / TPB) & 1) * 32;
+            if (at == 0) {
+                tab[lane] = next;
+                const int g = (j0 + i) * C::GROUPS + 32 + lane;
+                if (next.x < 0.0f && g - 32 < g_stop && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
+                next = scale_of(g, pg);
+                pg = page_of(g + 32);
+                __syncwarp();
+            }
+            const int sb = C::S2 ? i & 1 : 0;
+            if (!warp_wait(&s_full[2 * qtl + (i & 1)], (i >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const int kb = (j0 + i) * C::BN;
+            const uint32_t sbuf = lane_addr + sb * C::BN;
+            float s[C::BN];
+#pragma unroll
+            for (int cc = 0; cc < C::BN; cc += 32) tmem_ld32(sbuf + cc, s + cc);
+            float c[C::GROUPS], vmax = 0.0f;
+            bool hole = false;
+#pragma unroll
+            for (int g = 0; g < C::GROUPS; g++) {
+                c[g] = tab[at + g].x;
+                vmax = fmaxf(vmax, tab[at + g].y);
+                hole |= c[g] < 0.0f;
+            }
+            tmem_wait_ld();
+            if (__any_sync(0xffffffffu, hole || kb < lo || kb + C::BN > hi)) {
+#pragma unroll
+                for (int k = 0; k < C::BN; k++)
+                    if (kb + k < lo || kb + k >= hi || c[k / 16] < 0.0f) s[k] = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < C::GROUPS; g++) c[g] = fabsf(c[g]);
+            }
+            float mt = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < C::GROUPS; g++) {
+                float x = s[16 * g];
+#pragma unroll
+                for (int k = 1; k < 16; k++) x = fmaxf(x, s[16 * g + k]);
+                mt = fmaxf(mt, x * c[g]);
+            }
+            if (__any_sync(0xffffffffu, mt > m + kLazyLog2) || vmax > 4.0f * vref) {
+                const float mn = fmaxf(m, mt);
+                float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+                m = mn;
+                l2 = make_float2(l2.x * f, l2.y * f);
+                if (vmax > vref) {
+                    f *= vref / vmax;
+                    vref = vmax;
+                }
+                if (i > 0) {
+                    if (!warp_wait(&o_done[2 * qtl + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int cc = 0; cc < HD; cc += 32) {
+                        float o[32];
+                        tmem_ld32(lane_addr + C::SCOLS + cc, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] *= f;
+                        tmem_st32(lane_addr + C::SCOLS + cc, o);
+                    }
+                }
+            }
+            const float mneg = m == -INFINITY ? 0.0f : -m;
+            const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f;
+            const float2 mm = make_float2(mneg, mneg);
+#pragma unroll
+            for (int cc = 0; cc < C::BN; cc += 64) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const float cg = c[cc / 16 + g], w = tab[at + cc / 16 + g].y * vinv;
+                    const float2 c2 = make_float2(cg, cg), w2 = make_float2(w, w);
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        const float2 x = fma2(make_float2(s[cc + 16 * g + k], s[cc + 16 * g + k + 1]), c2, mm);
+                        const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                        l2 = add2(l2, p);
+                        const float2 y = mul2(p, w2);
+                        pk[8 * g + k / 2] = pack_h2(y.x, y.y);
+                    }
+                }
+                tmem_st32(sbuf + cc / 2, reinterpret_cast<const float*>(pk));
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * qtl + (i & 1)]);
+        }
+        if (n_mine > 0 && ok && !warp_wait(&o_done[2 * qtl + ((n_mine - 1) & 1)], ((n_mine - 1) >> 1) & 1, a.err, abort_flag))
+            ok = false;
+        tc_fence_after();
+        const bool have = n_mine > 0 && ok;
+        const float l = l2.x + l2.y;
+        auto load_o = [&](int cc, float* o, float f) {
+            if (have) {
+                tmem_ld32(lane_addr + C::SCOLS + cc, o);
+                tmem_wait_ld();
+            }
+#pragma unroll
+            for (int k = 0; k < 32; k++) o[k] = have ? o[k] * f : 0.0f;
+        };
+        const size_t orow = ((size_t)(rq.x + tok) * a.n_head + hd) * HD;
+        auto store = [&](int cc, const float* o, float f) {
+            if (!live) return;
+            if (a.out_type == SV_TYPE_F32) {
+                float4* d = reinterpret_cast<float4*>(static_cast<float*>(a.out) + orow + cc);
+#pragma unroll
+                for (int k = 0; k < 8; k++) d[k] = make_float4(o[4 * k] * f, o[4 * k + 1] * f, o[4 * k + 2] * f, o[4 * k + 3] * f);
+            } else {
+                uint4* d = reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + orow + cc);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    d[k] = make_uint4(pack_h2(o[8 * k] * f, o[8 * k + 1] * f), pack_h2(o[8 * k + 2] * f, o[8 * k + 3] * f),
+                                      pack_h2(o[8 * k + 4] * f, o[8 * k + 5] * f), pack_h2(o[8 * k + 6] * f, o[8 * k + 7] * f));
+            }
+        };
+        if (ns == 1) {
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+            for (int cc = 0; cc < HD; cc += 32) {
+                float o[32];
+                load_o(cc, o, vref);
+                store(cc, o, inv);
+            }
+        } else {
+            // partials as [column / 4][row] float4: a warp's rows are one 512-byte access
+            const size_t unit = (size_t)item * NKV + h, first = (size_t)(item - split) * NKV + h;
+            float4* part = reinterpret_cast<float4*>(a.work + a.l.pre_part);
+            float2* mls = reinterpret_cast<float2*>(a.work + a.l.pre_ml);
+            float4* wo = part + unit * C::ROWS * (HD / 4);
+#pragma unroll 1
+            for (int cc = 0; cc < HD; cc += 32) {
+                float o[32];
+                load_o(cc, o, vref);
+                if (tile_live) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        wo[(size_t)(cc / 4 + k) * C::ROWS + flat] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                }
+            }
+            if (tile_live) mls[unit * C::ROWS + flat] = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
+            __threadfence();
+            asm volatile("barrier.sync 2, %0;" ::"n"(C::SM_WARPS * 32) : "memory");
+            if (threadIdx.x == 0) {
+                int* ticket = reinterpret_cast<int*>(a.work + a.l.tick) + (size_t)a.l.dec_cap * NKV + first;
+                const int last = atomicAdd(ticket, 1) == ns - 1;
+                if (last) *ticket = 0;                     // ready for the next layer
+                *s_last = last;
+            }
+            asm volatile("barrier.sync 2, %0;" ::"n"(C::SM_WARPS * 32) : "memory");
+            if (*s_last && tile_live) {
+                __threadfence();
+                const size_t so = (size_t)NKV * C::ROWS;
+                const float2* ml = mls + first * C::ROWS + flat;
+                float M = -INFINITY, L = 0.0f;
+                for (int sp = 0; sp < ns; sp++) M = fmaxf(M, __ldcg(ml + sp * so).x);
+                for (int sp = 0; sp < ns; sp++) {
+                    const float2 x = __ldcg(ml + sp * so);
+                    L += x.x == -INFINITY ? 0.0f : x.y * fast_exp2(x.x - M);
+                }
+                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll 1
+                for (int cc = 0; cc < HD; cc += 32) {
+                    float o[32];
+#pragma unroll
+                    for (int k = 0; k < 32; k++) o[k] = 0.0f;
+                    for (int sp = 0; sp < ns; sp++) {
+                        const float x = __ldcg(ml + sp * so).x, w = x == -INFINITY ? 0.0f : fast_exp2(x - M);
+                        const float4* p = part + (first + (size_t)sp * NKV) * C::ROWS * (HD / 4) + (size_t)(cc / 4) * C::ROWS + flat;
+                        float4 v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] = __ldcg(p + (size_t)k * C::ROWS);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            o[4 * k] = fmaf(w, v[k].x, o[4 * k]);
+                            o[4 * k + 1] = fmaf(w, v[k].y, o[4 * k + 1]);
+                            o[4 * k + 2] = fmaf(w, v[k].z, o[4 * k + 2]);
+                            o[4 * k + 3] = fmaf(w, v[k].w, o[4 * k + 3]);
+                        }
+                    }
+                    store(cc, o, inv);
+                }
+            }
+        }
+    } else if (warp < C::SM_WARPS + C::CV_WARPS) {
+        // ============================ converters: entry e is K (even) or V (odd) of tile e / 2
+        if constexpr (C::SPLIT_REGS) regs_down<80>();
+        const int t = threadIdx.x - C::SM_WARPS * 32;
+        constexpr int TPR = HD / 16;                        // threads per row, 16 codes each
+        constexpr int RPP = C::CV_WARPS * 32 / TPR;         // rows per pass
+        constexpr int PASSES = C::BN / RPP;
+        const int c16 = t % TPR, r0 = t / TPR;
+        // pages of 32 groups from the batch's first, and of the next 32 (a batch is whole tiles)
+        int b0 = j0 * C::GROUPS;
+        int p0 = page_of(b0 + lane), p1 = page_of(b0 + 32 + lane);
+        uint4 raw[PASSES];
+        auto fetch = [&](int e, int p) {
+            const int row = p * RPP + r0, key = (j0 + (e >> 1)) * C::BN + row;
+            const int page = __shfl_sync(0xffffffffu, p0, ((key >> 4) - b0) & 31);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (e < 2 * n && (key >> 4) < g_stop && valid(page)) {
+                const uint8_t* src = static_cast<const uint8_t*>((e & 1) ? a.kv.v : a.kv.k);
+                x = __ldg(reinterpret_cast<const uint4*>(
+                    src + ((((size_t)page * NKV + h) << lg) + (key & (a.kv.page_size - 1))) * HD + c16 * 16));
+            }
+            return x;
+        };
+        if (n > 0) {
+#pragma unroll
+            for (int p = 0; p < PASSES; p++) raw[p] = fetch(0, p);
+        }
+        for (int e = 0; e < 2 * n; e++) {
+            const int sl = e % C::NE;
+            if (e >= C::NE && !warp_wait(&empty[sl], ((e / C::NE) - 1) & 1, a.err, abort_flag)) break;
+            // the next entry's tile may start in the next batch of groups
+            if ((j0 + ((e + 1) >> 1)) * C::GROUPS - b0 >= 32) {
+                b0 += 32;
+                p0 = p1;
+                p1 = page_of(b0 + 32 + lane);
+            }
+            uint8_t* dst = smem + C::OFF_RING + sl * C::KV_B + (c16 >> 2) * C::KBOX;
+            const int ch = (c16 & 3) * 2, swap = (c16 >> 2) & 1;
+#pragma unroll
+            for (int p = 0; p < PASSES; p++) {
+                const int row = p * RPP + r0;
+                const uint32_t w[4] = {raw[p].x ^ 0x80808080u, raw[p].y ^ 0x80808080u, raw[p].z ^ 0x80808080u, raw[p].w ^ 0x80808080u};
+                raw[p] = fetch(e + 1, p);
+                uint4 y[2];
+                y[0] = make_uint4(code_pair(w[0], 0x4140), code_pair(w[0], 0x4342), code_pair(w[1], 0x4140), code_pair(w[1], 0x4342));
+                y[1] = make_uint4(code_pair(w[2], 0x4140), code_pair(w[2], 0x4342), code_pair(w[3], 0x4140), code_pair(w[3], 0x4342));
+                // the eight threads of a store cover eight different 16-byte columns: half of them start with the second
+                uint8_t* base = dst + row * 128;
+                *reinterpret_cast<uint4*>(base + (((ch + swap) ^ (row & 7)) << 4)) = swap ? y[1] : y[0];
+                *reinterpret_cast<uint4*>(base + (((ch + 1 - swap) ^ (row & 7)) << 4)) = swap ? y[0] : y[1];
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[sl]);
+        }
+    } else {
+        if constexpr (C::SPLIT_REGS) regs_down<48>();
+        if (warp == C::SM_WARPS + C::CV_WARPS && lane == 0 && n > 0) {
+        // ============================ MMA issuer
+        const uint32_t idesc_s = umma_idesc(128, C::BN, 0, 0), idesc_o = umma_idesc(128, HD, 0, 1);
+        constexpr uint32_t hi = desc_hi_sw128(1024);
+        const uint32_t q_lo = desc_lo(smem_u32(smem), 16);
+        const uint32_t k_lo = desc_lo(smem_u32(smem + C::OFF_RING), 16);
+        const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_RING), C::KBOX);
+        auto wait_full = [&](int e) {
+            const bool r = wait_or_abort(&full[e % C::NE], (e / C::NE) & 1, a.err, abort_flag);
+            tc_fence_after();
+            return r;
+        };
+        auto mma_s = [&](int i, int q) {
+            const uint32_t kd = k_lo + (uint32_t)(((2 * i) % C::NE) * (C::KV_B >> 4));
+            const uint32_t d = tmem + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++) {
+                const uint32_t a_off = (uint32_t)((q * C::Q_B + (kk / 4) * C::QBOX + (kk % 4) * 32) >> 4);
+                const uint32_t b_off = (uint32_t)(((kk / 4) * C::KBOX + (kk % 4) * 32) >> 4);
+                umma_f16_w(d, q_lo + a_off, kd + b_off, hi, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[2 * q + (i & 1)]);
+        };
+        auto mma_pv = [&](int i, int q) -> bool {
+            if (!wait_or_abort(&p_full[2 * q + (i & 1)], (i >> 1) & 1, a.err, abort_flag)) return false;
+            tc_fence_after();
+            const uint32_t vd = v_lo + (uint32_t)(((2 * i + 1) % C::NE) * (C::KV_B >> 4));
+            const uint32_t p = tmem + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0), o = tmem + q * C::QCOLS + C::SCOLS;
+#pragma unroll
+            for (int kk = 0; kk < C::BN / 16; kk++)
+                umma_f16_ts(o, p + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), hi, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&o_done[2 * q + (i & 1)]);
+            return true;
+        };
+        bool ok = wait_or_abort(q_full, 0, a.err, abort_flag) && wait_full(0);
+        if (ok) {
+            for (int q = 0; q < nqt; q++) mma_s(0, q);
+            umma_commit(&empty[0]);
+        }
+        for (int i = 0; ok && i < n; i++) {
+            if (C::S2 && i + 1 < n) {                       // S(i+1) overlaps the softmax of tile i
+                ok = wait_full(2 * i + 2);
+                if (!ok) break;
+                mma_s(i + 1, 0);
+                umma_commit(&empty[(2 * i + 2) % C::NE]);
+            }
+            ok = wait_full(2 * i + 1);
+            for (int q = 0; q < nqt && ok; q++) {
+                ok = mma_pv(i, q);
+                if (!C::S2 && ok && i + 1 < n) {            // S_q(i+1) overwrites P_q(i), after P.V_q(i) on the same pipe
+                    if (q == 0) ok = wait_full(2 * i + 2);
+                    if (ok) mma_s(i + 1, q);
+                }
+            }
+            if (!ok) break;
+            umma_commit(&empty[(2 * i + 1) % C::NE]);
+            if (!C::S2 && i + 1 < n) umma_commit(&empty[(2 * i + 2) % C::NE]);
+        }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)C::TMEM_COLS));
+    }
+}
+
+template <int HD>
+cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
+    using C = PreCfgP<HD>;
+    constexpr int smem = C::SMEM + 1024;
+    static std::once_flag once[kMaxDevices];
+    static cudaError_t status[kMaxDevices];
+    const cudaError_t e = once_per_device(once, status, [] {
+        return cudaFuncSetAttribute(paged_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    });
+    if (e != cudaSuccess) return e;
+    return launch_pdl(paged_prefill_kernel<HD>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)), dim3(C::THREADS), (size_t)smem, st, a);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_prefill(const PagedAttn& a, cudaStream_t st) {
     if (a.l.pre_cap == 0) return cudaSuccess;
-    const dim3 grid((unsigned)(((int64_t)a.n_tokens * a.n_head + 7) / 8));
-    if (a.kv.head_dim == 64) return launch_pdl(paged_attn_kernel<64>, grid, dim3(256), 0, st, a);
-    if (a.kv.head_dim == 128) return launch_pdl(paged_attn_kernel<128>, grid, dim3(256), 0, st, a);
-    return launch_pdl(paged_attn_kernel<256>, grid, dim3(256), 0, st, a);
+    switch (a.kv.head_dim) {
+        case 64: return launch_hd<64>(a, st);
+        case 128: return launch_hd<128>(a, st);
+        default: return launch_hd<256>(a, st);
+    }
 }
 
 }  // namespace svkv
