@@ -198,10 +198,22 @@ def _ptr(x):
     return x.data_ptr()
 
 
+_torch_module = None
+
+
+def _torch():
+    """torch, imported on first use (the host-only entry points work without it)."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
+
+
 def _stream(stream):
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        # the current stream's handle without building a Stream object (3 us a call)
+        return _torch()._C._cuda_getCurrentRawStream(_torch()._C._cuda_getDevice())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -377,7 +389,7 @@ class KvCache:
 # =================================================================== paged 8-bit cache
 def _float_type(fn: str, t) -> int:
     """SV type id of an f16 or f32 tensor."""
-    import torch
+    torch = _torch()
     if t.dtype == torch.float16:
         return TYPE_F16
     if t.dtype == torch.float32:
@@ -388,6 +400,10 @@ def _float_type(fn: str, t) -> int:
 def _packed(t, heads: int, hd: int) -> bool:
     """[T, heads, hd] with a token's heads side by side."""
     return t.dim() == 3 and t.shape[1] == heads and t.shape[2] == hd and t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd)
+
+
+def _weights(w, hd: int) -> bool:
+    return w is None or (w.dtype == _torch().float32 and w.is_contiguous() and w.numel() == hd)
 
 
 def _row_bytes(t) -> int:
@@ -439,7 +455,7 @@ class PagedStep:
 
     def __init__(self, n_req: int, n_tokens: int, max_new: int, page_size: int, n_pages: int, n_head: int,
                  n_kv_head: int, head_dim: int, device: int = 0):
-        import torch
+        torch = _torch()
         self._s = s = _PagedStep(n_req, n_tokens, max_new, 1, n_head, n_kv_head, head_dim, page_size, n_pages)
         self._ref = ctypes.byref(s)
         s.work_bytes = lib().sv_paged_step_bytes(self._ref)
@@ -449,6 +465,7 @@ class PagedStep:
         new = lambda n: torch.zeros(n, dtype=torch.int32, device=dev)  # noqa: E731
         self.q_start, self.kv_len, self.n_free, self.err = new(n_req + 1), new(n_req), new(1), new(1)
         self.tok_req, self.tok_pos, self.tok_slot = new(n_tokens), new(n_tokens), new(n_tokens)
+        self._n_free_ptr = self.n_free.data_ptr()
         self.work = torch.empty(s.work_bytes, dtype=torch.uint8, device=dev)
         for name in ("q_start", "kv_len", "tok_req", "tok_pos", "tok_slot", "work", "err"):
             setattr(s, name, getattr(self, name).data_ptr())
@@ -458,9 +475,8 @@ class PagedStep:
         """Page tables, slot map and work lists of the step (sv_paged_plan): n_past, n_new int32 [n_req],
         table int32 [n_req, max_blocks] (new pages are written into it), free_pages int32 with *n_free pages.
         self.n_free gets what is left of them."""
-        import torch
-        i32 = torch.int32
-        _require("sv_paged_plan", n_past.dtype == n_new.dtype == table.dtype == free_pages.dtype == n_free.dtype == i32
+        torch = _torch()
+        _require("sv_paged_plan", n_past.dtype == n_new.dtype == table.dtype == free_pages.dtype == n_free.dtype == torch.int32
                  and table.is_contiguous() and n_past.is_contiguous() and n_new.is_contiguous()
                  and free_pages.is_contiguous() and table.dim() == 2 and table.shape[0] == self.n_req
                  and n_past.numel() == n_new.numel() == self.n_req)
@@ -468,8 +484,8 @@ class PagedStep:
         s.max_blocks = table.shape[1]
         s.n_past, s.n_new, s.table = n_past.data_ptr(), n_new.data_ptr(), table.data_ptr()
         self._keep = (n_past, n_new, table)
-        _check("sv_paged_plan", lib().sv_paged_plan(self._ref, free_pages.data_ptr(), n_free.data_ptr(),
-                                                    self.n_free.data_ptr(), _stream(stream)))
+        _check("sv_paged_plan", _lib.sv_paged_plan(self._ref, free_pages.data_ptr(), n_free.data_ptr(), self._n_free_ptr,
+                                                   _stream(stream)))
 
     def error_flags(self) -> int:
         """DEVERR_* bits raised by plans of this step since the last call (waits for them)."""
@@ -484,7 +500,7 @@ class PagedKv:
     [n_pages, n_kv_head, page_size, head_dim] with one f32 scale for each page and kv head (sv_paged)."""
 
     def __init__(self, n_layer: int, n_kv_head: int, head_dim: int, page_size: int, n_pages: int, device: int = 0):
-        import torch
+        torch = _torch()
         dev = torch.device("cuda", device)
         self.n_layer, self.n_kv_head, self.head_dim, self.page_size, self.n_pages = n_layer, n_kv_head, head_dim, page_size, n_pages
         self._codes = torch.zeros((n_layer, 2, n_pages, n_kv_head, page_size, head_dim), dtype=torch.int8, device=dev)
@@ -509,7 +525,7 @@ class PagedKv:
         k and v [T, n_kv_head, HD], all f16 or all f32, heads packed, any token stride of 16-byte multiples
         (views of one projection's output).  pos: int32 [T] ([4, T] for ROPE_IMROPE), or None: the plan's
         positions.  Returns the rotated queries (f16 unless q_out is given)."""
-        import torch
+        torch = _torch()
         fn, T = "sv_paged_append", step.n_tokens
         if q_out is None:
             q_out = torch.empty((T, step.n_head, step.head_dim), dtype=torch.float16, device=q.device)
@@ -519,18 +535,17 @@ class PagedKv:
                  and _packed(q, step.n_head, hd) and _packed(k, self.n_kv_head, hd) and _packed(v, self.n_kv_head, hd)
                  and (pos is None or (pos.dtype == torch.int32 and pos.is_contiguous()
                                       and pos.numel() == (4 * T if rope is not None and rope.mode == ROPE_IMROPE else T)))
-                 and all(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == hd)
-                         for w in (q_norm, k_norm)))
+                 and _weights(q_norm, hd) and _weights(k_norm, hd))
         r = _PagedRows(q.data_ptr(), k.data_ptr(), v.data_ptr(), _float_type(fn, q), _row_bytes(q), _row_bytes(k),
                        _row_bytes(v), _ptr(q_norm), _ptr(k_norm), eps, None if rope is None else rope.h, _ptr(pos),
                        q_out.data_ptr(), _float_type(fn, q_out))
-        _check(fn, lib().sv_paged_append(self._refs[layer], step._ref, ctypes.byref(r), _stream(stream)))
+        _check(fn, _lib.sv_paged_append(self._refs[layer], step._ref, ctypes.byref(r), _stream(stream)))
         return q_out
 
     def read(self, layer: int, slots, k_out=None, v_out=None, stream=None):
         """Rows of the cache as numbers (sv_paged_read): slots int32 [n] (page * page_size + offset) ->
         k, v [n, n_kv_head, head_dim], f16 unless outputs are given."""
-        import torch
+        torch = _torch()
         fn = "sv_paged_read"
         shape = (slots.numel(), self.n_kv_head, self.head_dim)
         if k_out is None:
@@ -539,7 +554,7 @@ class PagedKv:
             v_out = torch.empty(shape, dtype=k_out.dtype, device=slots.device)
         _require(fn, slots.dtype == torch.int32 and slots.is_contiguous() and k_out.shape == v_out.shape == shape
                  and k_out.dtype == v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous())
-        _check(fn, lib().sv_paged_read(self._refs[layer], slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
+        _check(fn, _lib.sv_paged_read(self._refs[layer], slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
                                        _float_type(fn, k_out), _stream(stream)))
         return k_out, v_out
 
@@ -547,13 +562,13 @@ class PagedKv:
         """Causal attention of the step's rows q [T, n_head, HD] (f16/f32, heads packed) over the pages
         (sv_paged_attn); window > 0: the last `window` positions only.  Returns [T, n_head, HD] f16 unless
         out is given."""
-        import torch
+        torch = _torch()
         fn = "sv_paged_attn"
         if out is None:
             out = torch.empty((step.n_tokens, step.n_head, step.head_dim), dtype=torch.float16, device=q.device)
         _require(fn, q.shape == out.shape == (step.n_tokens, step.n_head, self.head_dim)
                  and _packed(q, step.n_head, self.head_dim) and out.is_contiguous())
-        _check(fn, lib().sv_paged_attn(self._refs[layer], step._ref, q.data_ptr(), _float_type(fn, q),
+        _check(fn, _lib.sv_paged_attn(self._refs[layer], step._ref, q.data_ptr(), _float_type(fn, q),
                                        _row_bytes(q), scale, window, out.data_ptr(),
                                        _float_type(fn, out), _stream(stream)))
         return out
@@ -561,11 +576,11 @@ class PagedKv:
     def release(self, table, req, kv_len, free_pages, n_free, stream=None) -> None:
         """Pages of the requests `req` (rows of table, holding kv_len[i] tokens) back to the free list
         (sv_paged_release)."""
-        import torch
+        torch = _torch()
         fn = "sv_paged_release"
         _require(fn, all(t.dtype == torch.int32 and t.is_contiguous() for t in (table, req, kv_len, free_pages, n_free))
                  and req.numel() == kv_len.numel() and free_pages.numel() >= self.n_pages)
-        _check(fn, lib().sv_paged_release(table.data_ptr(), table.shape[0], table.shape[1], self.page_size, self.n_pages,
+        _check(fn, _lib.sv_paged_release(table.data_ptr(), table.shape[0], table.shape[1], self.page_size, self.n_pages,
                                           req.data_ptr(), req.numel(), kv_len.data_ptr(), free_pages.data_ptr(),
                                           n_free.data_ptr(), self.err.data_ptr(), _stream(stream)))
 

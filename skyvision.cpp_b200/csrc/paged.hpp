@@ -21,7 +21,10 @@
 
 namespace svkv {
 
-constexpr int kDecRows = 16;      // query rows of one decode unit (the M of its MMA)
+constexpr int kDecRows = 16;      // most query rows of one decode unit
+// Requests of up to this many rows are decode units: the eight-row kernel where the step's bounds allow no more or
+// a prefill kernel runs beside it anyway, else the sixteen-row one (one decode launch either way).
+inline int few_rows(int64_t most_rows) { return most_rows <= 8 || most_rows > kDecRows ? 8 : kDecRows; }
 constexpr int kDecTile = 64;      // keys per decode tile
 // decode CTAs that one SM holds (shared memory: a ring of K and V tiles each)
 constexpr int dec_ctas_per_sm(int hd) { return hd == 256 ? 2 : 3; }
@@ -35,6 +38,7 @@ enum : int { PH_PAGES = 0, PH_DEC = 1, PH_PRE = 2 };
 
 struct StepLayout {
     int page_cap = 0, dec_cap = 0, pre_cap = 0;     // most entries of each list
+    int few = kDecRows;                             // rows of a decode unit, at most
     int dec_slots = 1, pre_slots = 1;               // items that run at once, per kv head
     size_t head = 0, req = 0, page = 0, dec = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
     size_t bytes = 0;
@@ -63,7 +67,7 @@ struct PagedAttn {
     sv_paged kv;
     const int32_t* table;
     int max_blocks;
-    int n_req, n_tokens, max_new, n_head, G;
+    int n_req, n_tokens, n_head, G;
     const uint8_t* q;
     int q_type;
     size_t q_nb;

@@ -118,7 +118,6 @@ int sv_paged_attn(const sv_paged* kv, const sv_paged_step* step, const void* q, 
     a.max_blocks = step->max_blocks;
     a.n_req = step->n_req;
     a.n_tokens = step->n_tokens;
-    a.max_new = step->max_new;
     a.n_head = step->n_head;
     a.G = step->n_head / step->n_kv_head;
     a.q = static_cast<const uint8_t*>(q);

@@ -116,7 +116,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     const int split = it.y & 0xffff, ns = it.y >> 16;
     const int4 rq = reinterpret_cast<const int4*>(a.work + a.l.req)[it.x];   // first row, rows, held before, after
     const int rows = rq.y * a.G;
-    if ((rows > 8) != (NT == 2)) return;
     const int lo_key = a.window > 0 ? max(0, rq.z - a.window + 1) : 0;
     const int t_lo = lo_key / kDecTile, t_hi = (rq.w + kDecTile - 1) / kDecTile;
     const int nt_all = max(0, t_hi - t_lo);
@@ -496,13 +495,8 @@ cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
         !encode_tmap_2d(&tmv, a.kv.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz))
         return cudaErrorInvalidValue;
     const dim3 grid((unsigned)(a.l.dec_cap * a.kv.n_kv_head));
-    // Requests of up to 8 rows and of 9 to 16 take different kernels; either launch is left out where the
-    // step's bounds rule its requests out.
-    cudaError_t rc = cudaSuccess;
-    if (a.G <= 8) rc = launch_pdl(paged_decode_kernel<HD, 1>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
-    if (rc == cudaSuccess && (int64_t)a.max_new * a.G > 8)
-        rc = launch_pdl(paged_decode_kernel<HD, 2>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
-    return rc;
+    if (a.l.few <= 8) return launch_pdl(paged_decode_kernel<HD, 1>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
+    return launch_pdl(paged_decode_kernel<HD, 2>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
 }
 
 }  // namespace

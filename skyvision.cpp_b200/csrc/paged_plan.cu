@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
             const int held = (p + ps - 1) >> lg, want = min((p + c + ps - 1) >> lg, s.max_blocks);
             *np = max(want - held, 0);
             *nt = c > 0 ? ((p + c - 1) >> lg) - (p >> lg) + 1 : 0;
-            *ql = c * a.G > kDecRows ? (c * a.G + rows_per_unit - 1) / rows_per_unit : 0;
+            *ql = c * a.G > a.l.few ? (c * a.G + rows_per_unit - 1) / rows_per_unit : 0;
         };
         for (int r = r0; r < r1; r++) {
             int np, nt, ql;
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
         int2* dec = reinterpret_cast<int2*>(work + a.l.dec);
         auto dec_cost = [&](int r) {
             const int c = start[r + 1] - start[r];
-            if (c == 0 || c * a.G > kDecRows) return 0;
+            if (c == 0 || c * a.G > a.l.few) return 0;
             return (past[r] + c + kDecTile - 1) / kDecTile;
         };
         int base = 0;
@@ -313,12 +313,13 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     l->page_cap = (int)(T < T / ps + 2 * act ? T : T / ps + 2 * act);
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     l->dec_slots = (int)up((int64_t)sms * dec_ctas_per_sm(s.head_dim), s.n_kv_head);
-    l->dec_cap = G <= kDecRows ? (int)(act + l->dec_slots) : 0;
+    l->few = few_rows((int64_t)max_new * G);
+    l->dec_cap = G <= l->few ? (int)(act + l->dec_slots) : 0;
     l->pre_slots = (int)up(sms, s.n_kv_head);
     const int rows = pre_rows(s.head_dim);
-    if ((int64_t)max_new * G > kDecRows) {
-        const int64_t few = kDecRows / G + 1;    // fewest rows of a prefill request
-        l->pre_cap = (int)(T * G / rows + (act < T / few ? act : T / few) + l->pre_slots);
+    if ((int64_t)max_new * G > l->few) {
+        const int64_t least = l->few / G + 1;    // fewest tokens of a prefill request
+        l->pre_cap = (int)(T * G / rows + (act < T / least ? act : T / least) + l->pre_slots);
     }
     size_t at = 0;
     auto take = [&](size_t bytes) {
