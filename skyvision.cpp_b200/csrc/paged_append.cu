@@ -46,7 +46,8 @@ struct AppendArgs {
     int T, NH, G;
     const int4* pages;
     const int* head;
-    int kv_per;               // kv heads per block
+    int kv_per, kv_groups;    // kv heads per block, and blocks for them
+    int q_per;                // query heads per block (many rows)
     void* q_out;
     bool q_out_f32;
 };
@@ -55,27 +56,21 @@ template <bool F32>
 struct Raw8 { uint4 w[F32 ? 2 : 1]; };
 
 template <bool F32>
-__device__ __forceinline__ Raw8<F32> fetch8(const uint8_t* row, int e) {
+__device__ __forceinline__ Raw8<F32> fetch8(const uint8_t* at) {
     Raw8<F32> r;
-    const uint4* p = reinterpret_cast<const uint4*>(row + (size_t)e * (F32 ? 4 : 2));
+    const uint4* p = reinterpret_cast<const uint4*>(at);
     r.w[0] = p[0];
     if constexpr (F32) r.w[1] = p[1];
     return r;
 }
 
 template <bool F32>
-__device__ __forceinline__ void to_f32(const Raw8<F32>& r, float* x) {
+__device__ __forceinline__ void to_f32(const Raw8<F32>& r, float2* x) {
     const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
-    if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
+    for (int i = 0; i < 4; i++) {
+        if constexpr (F32) x[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else x[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     }
 }
 
@@ -85,14 +80,14 @@ __device__ __forceinline__ float load1(const uint8_t* row, int e) {
     else return __half2float(*reinterpret_cast<const __half*>(row + (size_t)e * 2));
 }
 
-__device__ __forceinline__ void store8(void* out, size_t at, bool f32, const float* x) {
+__device__ __forceinline__ void store8(void* out, size_t at, bool f32, const float2* x) {
     if (f32) {
         float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-        o[0] = make_float4(x[0], x[1], x[2], x[3]);
-        o[1] = make_float4(x[4], x[5], x[6], x[7]);
+        o[0] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+        o[1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
     } else {
         *reinterpret_cast<uint4*>(static_cast<__half*>(out) + at) =
-            make_uint4(pack_h2(x[0], x[1]), pack_h2(x[2], x[3]), pack_h2(x[4], x[5]), pack_h2(x[6], x[7]));
+            make_uint4(pack_h2(x[0].x, x[0].y), pack_h2(x[1].x, x[1].y), pack_h2(x[2].x, x[2].y), pack_h2(x[3].x, x[3].y));
     }
 }
 
@@ -100,10 +95,10 @@ __device__ __forceinline__ void store8(void* out, size_t at, bool f32, const flo
 // either side of a quarter; there the Taylor series to x^9 and x^8 are exact to f32 (next terms below 2^-25).
 __device__ __forceinline__ float2 turn(const float4 f, int pos, float mag) {
     const float p = (float)pos;
-    const float rest = (float)(int)((long long)pos - (long long)p);   // 0 below 2^24
     const float t = p * f.x, e = fmaf(p, f.x, -t);
     float r = t - rintf(t);
-    r += fmaf(p, f.y, e) + rest * f.x;
+    r += fmaf(p, f.y, e);
+    if (pos >= 1 << 24) r += (float)((long long)pos - (long long)p) * f.x;   // what p lost
     const float q = rintf(4.0f * r);
     const float a = fmaf(-0.25f, q, r) * 6.28318530717958647693f, a2 = a * a;
     const float sn = mag * a * fmaf(a2, fmaf(a2, fmaf(a2, fmaf(a2, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
@@ -115,127 +110,123 @@ __device__ __forceinline__ float2 turn(const float4 f, int pos, float mag) {
 
 // Factors of a thread's 8 elements [e, e + 8) and of their partners: y_i = x_i c_i + x'_i s_i.
 struct Rotation {
-    float c[8], s[8];
+    float2 c[4], s[4];
 };
 
+// Where an element's partner is.  ROT_OWN: with the same thread (pairs side by side; no rotation); ROT_RUN: eight
+// elements of another thread (halves of whole runs of eight); ROT_ANY: one by one.
+enum : int { ROT_OWN = 0, ROT_RUN = 1, ROT_ANY = 2 };
+
 // cs: the token's cosines [n_dims/2], then its sines.  w: norm weights or null.
+template <int ROT>
 __device__ __forceinline__ void rotation_of(const AppendArgs& a, const float* cs, int e, const float* w, Rotation* r) {
     const int half = a.n_dims >> 1;
-    const bool norm_mode = a.mode == SV_ROPE_NORM;
-    if (e >= a.n_dims) {
+    float c[8], s[8];
+    int pd[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            r->c[i] = w ? __ldg(w + e + i) : 1.0f;
-            r->s[i] = 0.0f;
-        }
-    } else if ((a.n_dims & 15) == 0) {             // whole runs of 8: 16-byte reads
-        if (norm_mode) {
-            const float4 c = *reinterpret_cast<const float4*>(cs + (e >> 1)), s = *reinterpret_cast<const float4*>(cs + half + (e >> 1));
-            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                r->c[i] = cc[i >> 1];
-                r->s[i] = i & 1 ? ss[i >> 1] : -ss[i >> 1];
-            }
-        } else {
-            const float4* c = reinterpret_cast<const float4*>(cs + (e < half ? e : e - half));
-            const float4* s = reinterpret_cast<const float4*>(cs + half + (e < half ? e : e - half));
+    for (int i = 0; i < 8; i++) c[i] = 1.0f, s[i] = 0.0f, pd[i] = e + i;
+    if constexpr (ROT == ROT_RUN) {
+        if (e < a.n_dims) {
+            const int p0 = e < half ? e : e - half;
             const float sg = e < half ? -1.0f : 1.0f;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float4 x = c[i], y = s[i];
-                r->c[4 * i] = x.x; r->c[4 * i + 1] = x.y; r->c[4 * i + 2] = x.z; r->c[4 * i + 3] = x.w;
-                r->s[4 * i] = sg * y.x; r->s[4 * i + 1] = sg * y.y; r->s[4 * i + 2] = sg * y.z; r->s[4 * i + 3] = sg * y.w;
+                const float4 x = *reinterpret_cast<const float4*>(cs + p0 + 4 * i);
+                const float4 y = *reinterpret_cast<const float4*>(cs + half + p0 + 4 * i);
+                c[4 * i] = x.x; c[4 * i + 1] = x.y; c[4 * i + 2] = x.z; c[4 * i + 3] = x.w;
+                s[4 * i] = sg * y.x; s[4 * i + 1] = sg * y.y; s[4 * i + 2] = sg * y.z; s[4 * i + 3] = sg * y.w;
             }
-        }
-        if (w) {
-            const int pe = norm_mode ? e : (e < half ? e + half : e - half);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                r->c[i] *= __ldg(w + e + i);
-                r->s[i] *= __ldg(w + pe + (norm_mode ? i ^ 1 : i));
-            }
+            for (int i = 0; i < 8; i++) pd[i] = (e < half ? e + half : e - half) + i;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int d = e + i;
-            float c = 1.0f, s = 0.0f;
-            int pd = d;
             if (d < a.n_dims) {
-                const bool second = norm_mode ? (i & 1) : d >= half;
-                const int pair = norm_mode ? d >> 1 : (second ? d - half : d);
-                pd = norm_mode ? d ^ 1 : (second ? d - half : d + half);
-                c = cs[pair];
-                s = second ? cs[half + pair] : -cs[half + pair];
+                const bool second = ROT == ROT_OWN ? (i & 1) : d >= half;
+                const int pair = ROT == ROT_OWN ? d >> 1 : (second ? d - half : d);
+                pd[i] = ROT == ROT_OWN ? e + (i ^ 1) : (second ? d - half : d + half);
+                c[i] = cs[pair];
+                s[i] = second ? cs[half + pair] : -cs[half + pair];
             }
-            r->c[i] = w ? c * __ldg(w + d) : c;
-            r->s[i] = w ? s * __ldg(w + pd) : s;
         }
     }
-}
-
-// The partners of a thread's elements, from the row again (L1) where they lie with another thread.
-enum : int { PART_NONE = 0, PART_OWN = 1, PART_VEC = 2, PART_ONE = 3 };
-__device__ __forceinline__ int partners_by(const AppendArgs& a, int e) {
-    if (e >= a.n_dims) return PART_NONE;
-    if (a.mode == SV_ROPE_NORM) return PART_OWN;
-    return (a.n_dims & 15) == 0 ? PART_VEC : PART_ONE;
-}
-__device__ __forceinline__ int partner_at(const AppendArgs& a, int e) {
-    const int half = a.n_dims >> 1;
-    return e < half ? e + half : e - half;
-}
-template <bool F32>
-__device__ __forceinline__ void partners(const AppendArgs& a, int by, const Raw8<F32>& pr, const uint8_t* row, int e, const float* x,
-                                         float* y) {
-    if (by == PART_VEC) {
-        to_f32<F32>(pr, y);
-    } else if (by == PART_OWN) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = x[i ^ 1];
-    } else {
-        const int half = a.n_dims >> 1;
+    if (w) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int d = e + i;
-            y[i] = by == PART_ONE && d < a.n_dims ? load1<F32>(row, d < half ? d + half : d - half) : 0.0f;
+            c[i] *= __ldg(w + e + i);
+            s[i] *= __ldg(w + pd[i]);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        r->c[i] = make_float2(c[2 * i], c[2 * i + 1]);
+        r->s[i] = make_float2(s[2 * i], s[2 * i + 1]);
     }
 }
 
 // 1 / rms over the row's lanes
 template <int HD>
-__device__ __forceinline__ float row_norm(const float* x, float eps) {
-    float ss = 0.0f;
+__device__ __forceinline__ float row_norm(const float2* x, float eps) {
+    float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < 4; i++) ss = fma2(x[i], x[i], ss);
+    float t = ss.x + ss.y;
 #pragma unroll
-    for (int o = HD / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    return 1.0f / sqrtf(ss / (float)HD + eps);
+    for (int o = HD / 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    return rsqrtf(t * (1.0f / HD) + eps);          // 2 units of 2^-23
 }
 
-template <int HD>
-__device__ __forceinline__ void apply(const AppendArgs& a, bool normed, const Rotation& r, const float* y, float* x) {
-    const float n = normed ? row_norm<HD>(x, a.eps) : 1.0f;
+// x = n (x c + x' s), n the row's norm; row points at this thread's first element (partners that are not the
+// thread's own are read from the row again, through L1: pr holds a run of eight)
+template <int HD, bool F32, int ROT>
+__device__ __forceinline__ void turn_row(const AppendArgs& a, bool normed, const Rotation& r, const Raw8<F32>& pr, const uint8_t* row,
+                                         int e, float2* x) {
+    float2 y[4];
+    // a dim past n_dims has no partner: 0, not s = 0 times a value that may not be a number
+    if constexpr (ROT == ROT_RUN) {
+        to_f32<F32>(pr, y);
+        if (e >= a.n_dims) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = n * fmaf(x[i], r.c[i], y[i] * r.s[i]);
+            for (int i = 0; i < 4; i++) y[i] = make_float2(0.0f, 0.0f);
+        }
+    } else if constexpr (ROT == ROT_OWN) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = e + 2 * i < a.n_dims ? make_float2(x[i].y, x[i].x) : make_float2(0.0f, 0.0f);
+    } else {
+        const int half = a.n_dims >> 1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = e + i;
+            const float v = d < a.n_dims ? load1<F32>(row, d < half ? i + half : i - half) : 0.0f;
+            if (i & 1) y[i >> 1].y = v;
+            else y[i >> 1].x = v;
+        }
+    }
+    const float n = normed ? row_norm<HD>(x, a.eps) : 1.0f;
+    const float2 nn = make_float2(n, n);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = mul2(fma2(x[i], r.c[i], mul2(y[i], r.s[i])), nn);
 }
 
 // ---- quantising
 // Running maximum of |x|, and NaN in *bad once a value is not finite (0 x is NaN then).
-__device__ __forceinline__ void watch(const float* x, float* amax, float* bad) {
+__device__ __forceinline__ void watch(const float2* x, float* amax, float2* bad) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        *amax = fmaxf(*amax, fabsf(x[i]));
-        *bad = fmaf(x[i], 0.0f, *bad);
+    for (int i = 0; i < 4; i++) {
+        *amax = fmaxf(fmaxf(*amax, fabsf(x[i].x)), fabsf(x[i].y));
+        *bad = fma2(x[i], make_float2(0.0f, 0.0f), *bad);
     }
 }
-__device__ __forceinline__ float finite_max(const float* x) {
+__device__ __forceinline__ bool is_bad(float2 b) { return b.x != 0.0f || b.y != 0.0f; }
+__device__ __forceinline__ float finite_max(const float2* x) {
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (fabsf(x[i]) <= 3.402823466e38f) m = fmaxf(m, fabsf(x[i]));
+    for (int i = 0; i < 4; i++) {
+        if (fabsf(x[i].x) <= 3.402823466e38f) m = fmaxf(m, fabsf(x[i].x));
+        if (fabsf(x[i].y) <= 3.402823466e38f) m = fmaxf(m, fabsf(x[i].y));
+    }
     return m;
 }
 __device__ __forceinline__ void page_scale(float amax, float s_old, float* s, float* inv) {
@@ -243,30 +234,37 @@ __device__ __forceinline__ void page_scale(float amax, float s_old, float* s, fl
     *s = fmaxf(s_old, __fdiv_rn(amax, 127.0f));
     *inv = *s > 0.0f ? __fdiv_rn(1.0f, *s) : 0.0f;
 }
-// Codes of 8 values, round-half-even of x inv: the sum with 1.5 2^23 leaves the integer in its low byte.
-// |x inv| is at most 127 (1 + 2^-23), which rounds to 127.
-__device__ __forceinline__ uint2 codes8(const float* x, float inv) {
+// Codes of 8 values, round-half-even of x inv: the sum with 1.5 2^23 leaves the integer in its low byte.  The
+// product is rounded by itself: its sum is taken one by one, since a packed product and a packed sum are fused
+// by the assembler into one rounding.  |x inv| is at most 127 (1 + 2^-23), which rounds to 127.
+__device__ __forceinline__ uint2 codes8(const float2* x, float inv) {
+    const float2 ii = make_float2(inv, inv);
+    const float magic = 12582912.0f;
     uint32_t w[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        uint32_t b[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[4 * j + i], inv), 12582912.0f));
-        w[j] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        const float2 p0 = mul2(x[2 * j], ii), p1 = mul2(x[2 * j + 1], ii);
+        w[j] = __byte_perm(__byte_perm(__float_as_uint(__fadd_rn(p0.x, magic)), __float_as_uint(__fadd_rn(p0.y, magic)), 0x0040),
+                           __byte_perm(__float_as_uint(__fadd_rn(p1.x, magic)), __float_as_uint(__fadd_rn(p1.y, magic)), 0x0040), 0x5410);
     }
     return make_uint2(w[0], w[1]);
 }
 // infinities to +-127, NaN to 0
-__device__ __forceinline__ void tame(float* x, float s) {
+__device__ __forceinline__ float tame1(float x, float s) {
+    return fabsf(x) <= 3.402823466e38f ? x : (x > 0.0f ? 127.0f * s : (x < 0.0f ? -127.0f * s : 0.0f));
+}
+__device__ __forceinline__ void tame(float2* x, float s) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (!(fabsf(x[i]) <= 3.402823466e38f)) x[i] = x[i] > 0.0f ? 127.0f * s : (x[i] < 0.0f ? -127.0f * s : 0.0f);
+    for (int i = 0; i < 4; i++) x[i] = make_float2(tame1(x[i].x, s), tame1(x[i].y, s));
 }
 // eight codes that the page holds, rounded to its new scale (f = s_old / s)
 __device__ __forceinline__ uint2 recode8(uint2 c, float f) {
-    float x[8];
+    float2 x[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)(int8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = i < 2 ? c.x : c.y;
+        x[i] = make_float2((float)(int8_t)(w >> (16 * (i & 1))), (float)(int8_t)(w >> (16 * (i & 1) + 8)));
+    }
     return codes8(x, f);
 }
 // rows [first, end) of a page, `step` apart, this thread's 8 codes of each
@@ -296,59 +294,88 @@ __device__ __forceinline__ void fill_turns(const AppendArgs& a, int t0, int rows
 }
 
 // ---------------- up to NV rows per page
-template <int HD, bool F32, int NV>
+template <int HD, bool F32, int ROT, int NV>
 __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const __grid_constant__ AppendArgs a) {
     constexpr int C = HD / 8, PER = 256 / C;       // threads per row, rows at once
     constexpr int ES = F32 ? 4 : 2;
-    extern __shared__ float cs[];
+    extern __shared__ __align__(16) float cs[];
     pdl_wait();
     if (threadIdx.x == 0) pdl_trigger();
-    if ((int)blockIdx.x >= a.head[PH_PAGES]) return;
     const int4 it = a.pages[blockIdx.x];           // first row, page, offset in it, rows
+    if ((int)blockIdx.x >= a.head[PH_PAGES]) return;
     const int n = min(it.w, NV);
     const int e = (threadIdx.x % C) * 8, u = threadIdx.x / C;
     const int kv0 = blockIdx.y * a.kv_per, kvn = min(a.kv_per, a.kv.n_kv_head - kv0);
+    const int units = it.y >= 0 ? 2 * kvn : 0;     // kv head i / 2, K or V; none without a page
+    const int q0 = kv0 * a.G, qn = kvn * a.G, q_rows = n * qn;
+    // offset of the partner run (0 where there is none)
+    const int half = a.n_dims >> 1;
+    const int poff = ROT == ROT_RUN && e < a.n_dims ? (e < half ? half : -half) * ES : 0;
+    // This thread's rows of a pass.  The first pass of both kinds is loaded before the sines are computed.
+    const uint8_t* kp = a.k + (size_t)it.x * a.k_nb + (size_t)kv0 * HD * ES + e * ES;
+    const uint8_t* vp = a.v + (size_t)it.x * a.v_nb + (size_t)kv0 * HD * ES + e * ES;
+    const uint8_t* qp = a.q + (size_t)it.x * a.q_nb + (size_t)q0 * HD * ES + e * ES;
+    auto unit_src = [&](int i) { return ((i & 1) == 0 ? kp : vp) + (i >> 1) * (HD * ES); };
+    Raw8<F32> raw[NV], praw[NV], qraw, qpraw;
+    float s_old = 0.0f;
+    auto load_unit = [&](int i) {
+        if (i >= units) return;
+        const uint8_t* src = unit_src(i);
+        const bool is_k = (i & 1) == 0;
+        const size_t nb = is_k ? a.k_nb : a.v_nb;
+        if (it.z > 0) s_old = (is_k ? a.kv.k_scale : a.kv.v_scale)[(size_t)it.y * a.kv.n_kv_head + kv0 + (i >> 1)];
+#pragma unroll
+        for (int r = 0; r < NV; r++)
+            if (r < n) {
+                raw[r] = fetch8<F32>(src + r * nb);
+                if (ROT == ROT_RUN && is_k) praw[r] = fetch8<F32>(src + r * nb + poff);
+            }
+    };
+    int qr = 0, qh = 0;                            // row and head of this thread's query row
+    const uint8_t* qrow = qp;
+    auto load_q = [&](int i) {
+        qr = NV == 1 ? 0 : i / qn;
+        qh = NV == 1 ? i : i - qr * qn;
+        if (i >= q_rows) qr = qh = 0;
+        qrow = qp + (size_t)qr * a.q_nb + qh * (HD * ES);
+        qraw = fetch8<F32>(qrow);
+        if (ROT == ROT_RUN) qpraw = fetch8<F32>(qrow + poff);
+    };
+    load_unit(u);
+    load_q(u);
     if (a.pairs) {
         fill_turns(a, it.x, n, cs);
         __syncthreads();
     }
-    const int by = partners_by(a, e);
-    // ---- units: kv head 2 i / 2, K or V
-    for (int i0 = 0; it.y >= 0 && i0 < 2 * kvn; i0 += PER) {
-        const bool live = i0 + u < 2 * kvn;
-        const int i = live ? i0 + u : 0;
-        const int h = kv0 + (i >> 1);
-        const bool is_k = (i & 1) == 0;
-        const uint8_t* src = (is_k ? a.k + (size_t)it.x * a.k_nb : a.v + (size_t)it.x * a.v_nb) + (size_t)h * HD * ES;
-        const size_t nb = is_k ? a.k_nb : a.v_nb;
-        const size_t unit = (size_t)it.y * a.kv.n_kv_head + h;
-        float* sp = (is_k ? a.kv.k_scale : a.kv.v_scale) + unit;
-        const float s_old = it.z > 0 ? *sp : 0.0f;
-        Raw8<F32> raw[NV], praw[NV];
-#pragma unroll
-        for (int r = 0; r < NV; r++)
-            if (r < n) {
-                raw[r] = fetch8<F32>(src + r * nb, e);
-                if (is_k && by == PART_VEC) praw[r] = fetch8<F32>(src + r * nb, partner_at(a, e));
-            }
-        float x[NV][8], amax = 0.0f, bad = 0.0f;
+    for (int i0 = 0; i0 < units; i0 += PER) {
+        const int i = i0 + u;
+        const bool live = i < units, is_k = live && (i & 1) == 0;
+        const size_t unit = (size_t)it.y * a.kv.n_kv_head + kv0 + ((live ? i : 0) >> 1);
+        float2 x[NV][4], bad = make_float2(0.0f, 0.0f);
+        float amax = 0.0f;
 #pragma unroll
         for (int r = 0; r < NV; r++) {
             if (r >= n) break;
-            to_f32<F32>(raw[r], x[r]);
-            // K and V rows share warps: the norm's shuffles run for both
-            const float nrm = a.kn ? row_norm<HD>(x[r], a.eps) : 1.0f;
-            if (is_k && (a.pairs || a.kn)) {
-                float y[8];
-                Rotation rot;
-                partners<F32>(a, by, praw[r], src + r * nb, e, x[r], y);
-                rotation_of(a, cs + r * a.n_dims, e, a.kn, &rot);
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[r][j] = nrm * fmaf(x[r][j], rot.c[j], y[j] * rot.s[j]);
+            for (int j = 0; j < 4; j++) x[r][j] = make_float2(0.0f, 0.0f);
+            if (live) to_f32<F32>(raw[r], x[r]);
+            if (a.pairs || a.kn) {
+                // K and V rows share warps: all go through (the norm's shuffles), K rows take the result
+                float2 y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[j] = x[r][j];
+                Rotation rot;
+                rotation_of<ROT>(a, cs + r * a.n_dims, e, a.kn, &rot);
+                turn_row<HD, F32, ROT>(a, a.kn != nullptr, rot, is_k ? praw[r] : raw[r], is_k ? unit_src(i) + r * a.k_nb : kp, e, y);
+                if (is_k) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[r][j] = y[j];
+                }
             }
             watch(x[r], &amax, &bad);
         }
-        if (__any_sync(0xffffffffu, bad != 0.0f)) {     // NaN
+        const bool odd = is_bad(bad);
+        if (__any_sync(0xffffffffu, odd)) {
             amax = 0.0f;
 #pragma unroll
             for (int r = 0; r < NV; r++)
@@ -360,203 +387,159 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
         page_scale(amax, s_old, &s, &inv);
         __syncwarp();                              // the row's threads have read the old scale
         if (live) {
-            if (e == 0) *sp = s;
+            if (e == 0) (is_k ? a.kv.k_scale : a.kv.v_scale)[unit] = s;
             uint8_t* page = static_cast<uint8_t*>(is_k ? a.kv.k : a.kv.v) + unit * a.kv.page_size * HD;
 #pragma unroll
             for (int r = 0; r < NV; r++)
                 if (r < n) {
-                    if (bad != 0.0f) tame(x[r], s);
+                    if (odd) tame(x[r], s);
                     *reinterpret_cast<uint2*>(page + (size_t)(it.z + r) * HD + e) = codes8(x[r], inv);
                 }
             if (s > s_old && it.z > 0) recode_rows<HD>(page, 0, it.z, 1, e, __fmul_rn(s_old, inv));
         }
+        load_unit(i + PER);
     }
-    // ---- query rows
-    const int q0 = kv0 * a.G, qn = kvn * a.G;
-    for (int i0 = 0; i0 < n * qn; i0 += PER) {
-        const bool live = i0 + u < n * qn;
-        const int i = live ? i0 + u : 0, r = i / qn, h = q0 + i - r * qn;
-        const uint8_t* row = a.q + (size_t)(it.x + r) * a.q_nb + (size_t)h * HD * ES;
-        float x[8];
-        const Raw8<F32> raw = fetch8<F32>(row, e);
-        Raw8<F32> praw;
-        if (by == PART_VEC) praw = fetch8<F32>(row, partner_at(a, e));
-        to_f32<F32>(raw, x);
+    for (int i0 = 0; i0 < q_rows; i0 += PER) {
+        float2 x[4];
+        to_f32<F32>(qraw, x);
         if (a.pairs || a.qn) {
-            float y[8];
             Rotation rot;
-            partners<F32>(a, by, praw, row, e, x, y);
-            rotation_of(a, cs + r * a.n_dims, e, a.qn, &rot);
-            apply<HD>(a, a.qn != nullptr, rot, y, x);
+            rotation_of<ROT>(a, cs + qr * a.n_dims, e, a.qn, &rot);
+            turn_row<HD, F32, ROT>(a, a.qn != nullptr, rot, qpraw, qrow, e, x);
         }
         __syncwarp();                              // q_out may be q: the row's partners have been read
-        if (live) store8(a.q_out, ((size_t)(it.x + r) * a.NH + h) * HD + e, a.q_out_f32, x);
+        if (i0 + u < q_rows) store8(a.q_out, ((size_t)(it.x + qr) * a.NH + q0 + qh) * HD + e, a.q_out_f32, x);
+        if (i0 + PER < q_rows) load_q(i0 + u + PER);
     }
 }
 
-// ---------------- up to NV x (THREADS / C) rows per page
-template <int HD, bool F32, int THREADS, int NV>
+// ---------------- up to NV x (THREADS / C) rows per page; K, V and the queries in blocks of their own
+template <int HD, bool F32, int ROT, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 3 : 2) paged_append_many(const __grid_constant__ AppendArgs a) {
     constexpr int C = HD / 8, RP = THREADS / C;    // threads per row, rows per pass
     constexpr int ES = F32 ? 4 : 2, W = THREADS / 32;
-    extern __shared__ float cs[];
-    __shared__ float s_max[2][2][W];               // [parity of the head][K, V]
-    __shared__ int s_bad[2];
+    extern __shared__ __align__(16) float cs[];
+    __shared__ float s_max[2][W];                  // by the parity of the head
+    __shared__ int s_bad[3];                       // head hi's at hi % 3: cleared a barrier before it is set again
     pdl_wait();
     if (threadIdx.x == 0) pdl_trigger();
-    if ((int)blockIdx.x >= a.head[PH_PAGES]) return;
     const int4 it = a.pages[blockIdx.x];
+    if ((int)blockIdx.x >= a.head[PH_PAGES]) return;
     const int n = min(it.w, NV * RP);
     const int e = (threadIdx.x % C) * 8, r0 = threadIdx.x / C;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kv0 = blockIdx.y * a.kv_per, kvn = min(a.kv_per, a.kv.n_kv_head - kv0);
-    const int by = partners_by(a, e);
-    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
-    if (a.pairs) fill_turns(a, it.x, n, cs);
-    __syncthreads();
-    for (int hi = 0; it.y >= 0 && hi < kvn; hi++) {
-        const int h = kv0 + hi, par = hi & 1;
-        const uint8_t* ks = a.k + (size_t)it.x * a.k_nb + (size_t)h * HD * ES;
-        const uint8_t* vs = a.v + (size_t)it.x * a.v_nb + (size_t)h * HD * ES;
-        const size_t unit = (size_t)it.y * a.kv.n_kv_head + h;
-        Raw8<F32> kr[NV], vr[NV];
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int r = r0 + i * RP;
-            if (r < n) {
-                kr[i] = fetch8<F32>(ks + (size_t)r * a.k_nb, e);
-                vr[i] = fetch8<F32>(vs + (size_t)r * a.v_nb, e);
-            }
-        }
-        const float k_old = it.z > 0 ? a.kv.k_scale[unit] : 0.0f, v_old = it.z > 0 ? a.kv.v_scale[unit] : 0.0f;
-        float x[NV][8], kmax = 0.0f, vmax = 0.0f, bad = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            if (i * RP >= n) break;
-            const int r = r0 + i * RP;
-            const bool live = r < n;
-            if (live) {
-                to_f32<F32>(kr[i], x[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[i][j] = 0.0f;
-            }
-            if (a.pairs || a.kn) {                 // whole warps go through (the norm's shuffles)
-                const int rr = live ? r : 0;
-                const uint8_t* row = ks + (size_t)rr * a.k_nb;
-                Raw8<F32> pr;
-                if (by == PART_VEC) pr = fetch8<F32>(row, partner_at(a, e));
-                float y[8];
-                Rotation rot;
-                partners<F32>(a, by, pr, row, e, x[i], y);
-                rotation_of(a, cs + rr * a.n_dims, e, a.kn, &rot);
-                apply<HD>(a, a.kn != nullptr, rot, y, x[i]);
-            }
-            if (live) {
-                watch(x[i], &kmax, &bad);
-                float v[8];
-                to_f32<F32>(vr[i], v);
-                watch(v, &vmax, &bad);
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-        }
-        if (lane == 0) {
-            s_max[par][0][warp] = kmax;
-            s_max[par][1][warp] = vmax;
-        }
-        if (__any_sync(0xffffffffu, bad != 0.0f) && lane == 0) s_bad[par] = 1;
-        __syncthreads();                           // maxima meet; every thread has read the old scales
-        if (s_bad[par]) {                          // once more over the finite values
-            kmax = vmax = 0.0f;
+    const int half = a.n_dims >> 1;
+    const int poff = ROT == ROT_RUN && e < a.n_dims ? (e < half ? half : -half) * ES : 0;
+    if ((int)blockIdx.y < 2 * a.kv_groups) {
+        const bool is_k = (blockIdx.y & 1) == 0;
+        const int kv0 = (blockIdx.y >> 1) * a.kv_per, kvn = min(a.kv_per, a.kv.n_kv_head - kv0);
+        if (it.y < 0) return;                      // no page: dropped (the plan raised the error)
+        const size_t nb = is_k ? a.k_nb : a.v_nb;
+        const uint8_t* src = (is_k ? a.k : a.v) + (size_t)(it.x + min(r0, n - 1)) * nb + (size_t)kv0 * HD * ES + e * ES;
+        float* scales = (is_k ? a.kv.k_scale : a.kv.v_scale) + (size_t)it.y * a.kv.n_kv_head + kv0;
+        uint8_t* pages = static_cast<uint8_t*>(is_k ? a.kv.k : a.kv.v) + ((size_t)it.y * a.kv.n_kv_head + kv0) * a.kv.page_size * HD;
+        const bool turned = is_k && (a.pairs || a.kn);
+        Raw8<F32> raw[NV];
+        auto load = [&](int hi) {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (r0 + i * RP < n) {
-                    float v[8];
-                    to_f32<F32>(vr[i], v);
-                    kmax = fmaxf(kmax, finite_max(x[i]));
-                    vmax = fmaxf(vmax, finite_max(v));
+                if (r0 + i * RP < n) raw[i] = fetch8<F32>(src + (size_t)(i * RP) * nb + hi * (HD * ES));
+        };
+        load(0);
+        if (threadIdx.x < 3) s_bad[threadIdx.x] = 0;
+        if (is_k && a.pairs) fill_turns(a, it.x, n, cs);
+        __syncthreads();
+        for (int hi = 0; hi < kvn; hi++) {
+            const int par = hi & 1, slot = hi % 3;
+            const float s_old = it.z > 0 ? scales[hi] : 0.0f;
+            float2 x[NV][4], bad = make_float2(0.0f, 0.0f);
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                if (i * RP >= n) break;
+                const bool live = r0 + i * RP < n;
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[i][j] = make_float2(0.0f, 0.0f);
+                if (live) to_f32<F32>(raw[i], x[i]);
+                if (turned) {                      // whole warps go through (the norm's shuffles); a dead row takes the first
+                    const uint8_t* row = src + (live ? (size_t)(i * RP) * nb : 0) + hi * (HD * ES);
+                    Raw8<F32> pr;
+                    if (ROT == ROT_RUN) pr = fetch8<F32>(row + poff);
+                    Rotation rot;
+                    rotation_of<ROT>(a, cs + (live ? r0 + i * RP : 0) * a.n_dims, e, a.kn, &rot);
+                    turn_row<HD, F32, ROT>(a, a.kn != nullptr, rot, pr, row, e, x[i]);
                 }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+                if (live) watch(x[i], &amax, &bad);
             }
-            __syncthreads();
-            if (lane == 0) {
-                s_max[par][0][warp] = kmax;
-                s_max[par][1][warp] = vmax;
+            if (hi + 1 < kvn) load(hi + 1);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            if (lane == 0) s_max[par][warp] = amax;
+            if (__any_sync(0xffffffffu, is_bad(bad)) && lane == 0) s_bad[slot] = 1;
+            if (threadIdx.x == 0) s_bad[(hi + 1) % 3] = 0;
+            __syncthreads();                       // maxima meet; every thread has read the old scale
+            const bool any_bad = s_bad[slot] != 0;
+            if (any_bad) {                         // once more over the finite values
+                amax = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+                    if (r0 + i * RP < n) amax = fmaxf(amax, finite_max(x[i]));
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                __syncthreads();
+                if (lane == 0) s_max[par][warp] = amax;
+                __syncthreads();
             }
-            __syncthreads();
-        }
-        const bool any_bad = s_bad[par] != 0;
-        kmax = vmax = 0.0f;
+            amax = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            kmax = fmaxf(kmax, s_max[par][0][w]);
-            vmax = fmaxf(vmax, s_max[par][1][w]);
-        }
-        if (threadIdx.x == 0) s_bad[par ^ 1] = 0;  // the next head's; its last reader is a barrier behind
-        float sk, ik, sv, iv;
-        page_scale(kmax, k_old, &sk, &ik);
-        page_scale(vmax, v_old, &sv, &iv);
-        if (threadIdx.x == 0) {
-            a.kv.k_scale[unit] = sk;
-            a.kv.v_scale[unit] = sv;
-        }
-        uint8_t* kp = static_cast<uint8_t*>(a.kv.k) + unit * a.kv.page_size * HD;
-        uint8_t* vp = static_cast<uint8_t*>(a.kv.v) + unit * a.kv.page_size * HD;
+            for (int w = 0; w < W; w++) amax = fmaxf(amax, s_max[par][w]);
+            float s, inv;
+            page_scale(amax, s_old, &s, &inv);
+            if (threadIdx.x == 0) scales[hi] = s;
+            uint8_t* page = pages + (size_t)hi * a.kv.page_size * HD;
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int r = r0 + i * RP;
-            if (r < n) {
-                float v[8];
-                to_f32<F32>(vr[i], v);
-                if (any_bad) {
-                    tame(x[i], sk);
-                    tame(v, sv);
+            for (int i = 0; i < NV; i++) {
+                const int r = r0 + i * RP;
+                if (r < n) {
+                    if (any_bad) tame(x[i], s);
+                    *reinterpret_cast<uint2*>(page + (it.z + r) * HD + e) = codes8(x[i], inv);
                 }
-                *reinterpret_cast<uint2*>(kp + (size_t)(it.z + r) * HD + e) = codes8(x[i], ik);
-                *reinterpret_cast<uint2*>(vp + (size_t)(it.z + r) * HD + e) = codes8(v, iv);
             }
+            if (it.z > 0 && s > s_old) recode_rows<HD>(page, r0, it.z, RP, e, __fmul_rn(s_old, inv));
         }
-        if (it.z > 0) {
-            if (sk > k_old) recode_rows<HD>(kp, r0, it.z, RP, e, __fmul_rn(k_old, ik));
-            if (sv > v_old) recode_rows<HD>(vp, r0, it.z, RP, e, __fmul_rn(v_old, iv));
-        }
+        return;
     }
-    // ---- query rows: a thread keeps its token and chunk over the heads
+    // ---- query rows: a thread keeps its token and chunk, and so its rotation, over the heads
     constexpr int U = F32 ? 2 : 4;                 // heads whose loads are in flight
-    const int q0 = kv0 * a.G, qe = q0 + kvn * a.G;
+    const int q0 = ((int)blockIdx.y - 2 * a.kv_groups) * a.q_per, qn = min(a.q_per, a.NH - q0);
     const bool turned = a.pairs || a.qn;
+    if (a.pairs) {
+        fill_turns(a, it.x, n, cs);
+        __syncthreads();
+    }
     for (int rb = 0; rb < n; rb += RP) {
         const bool live = rb + r0 < n;
-        const int t = it.x + (live ? rb + r0 : 0);
+        const int r = live ? rb + r0 : 0;
         Rotation rot;
-        if (turned) rotation_of(a, cs + (t - it.x) * a.n_dims, e, a.qn, &rot);
-        for (int hb = q0; hb < qe; hb += U) {
+        if (turned) rotation_of<ROT>(a, cs + r * a.n_dims, e, a.qn, &rot);
+        const uint8_t* row = a.q + (size_t)(it.x + r) * a.q_nb + (size_t)q0 * HD * ES + e * ES;
+        const size_t to = ((size_t)(it.x + r) * a.NH + q0) * HD + e;
+        for (int hb = 0; hb < qn; hb += U) {
             Raw8<F32> raw[U], pr[U];
 #pragma unroll
             for (int j = 0; j < U; j++) {
-                const uint8_t* row = a.q + (size_t)t * a.q_nb + (size_t)min(hb + j, qe - 1) * HD * ES;
-                raw[j] = fetch8<F32>(row, e);
-                if (by == PART_VEC) pr[j] = fetch8<F32>(row, partner_at(a, e));
+                const int off = min(hb + j, qn - 1) * (HD * ES);
+                raw[j] = fetch8<F32>(row + off);
+                if (ROT == ROT_RUN) pr[j] = fetch8<F32>(row + off + poff);
             }
             __syncwarp();                          // q_out may be q: these heads' partners have been read
 #pragma unroll
             for (int j = 0; j < U; j++) {
-                float x[8];
+                float2 x[4];
                 to_f32<F32>(raw[j], x);
-                if (turned) {
-                    float y[8];
-                    partners<F32>(a, by, pr[j], a.q + (size_t)t * a.q_nb + (size_t)min(hb + j, qe - 1) * HD * ES, e, x, y);
-                    apply<HD>(a, a.qn != nullptr, rot, y, x);
-                }
-                __syncwarp();                      // as above, for partners that were read one by one
-                if (live && hb + j < qe) store8(a.q_out, ((size_t)t * a.NH + hb + j) * HD + e, a.q_out_f32, x);
+                if (turned) turn_row<HD, F32, ROT>(a, a.qn != nullptr, rot, pr[j], row + min(hb + j, qn - 1) * (HD * ES), e, x);
+                if (ROT == ROT_ANY) __syncwarp();  // as above, for partners that were read one by one
+                if (live && hb + j < qn) store8(a.q_out, to + (hb + j) * HD, a.q_out_f32, x);
             }
         }
     }
@@ -575,7 +558,7 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const __grid_const
         const int slot = __ldg(slots + i);
         const bool ok = slot >= 0 && (slot >> lg) < kv.n_pages;
         if (!ok && slot != -1 && at == 0 && kv.err) atomicOr(kv.err, ERRBIT_ROW_RANGE);
-        float x[2][8] = {};
+        float2 x[2][4] = {};
         if (ok) {
             const size_t unit = (size_t)(slot >> lg) * kv.n_kv_head + h;
             const size_t off = (unit * kv.page_size + (slot & (kv.page_size - 1))) * kv.head_dim + e;
@@ -585,8 +568,10 @@ __global__ void __launch_bounds__(kThreads) paged_read_kernel(const __grid_const
 #pragma unroll
             for (int o = 0; o < 2; o++)
 #pragma unroll
-                for (int b = 0; b < 8; b++)
-                    x[o][b] = (float)(int8_t)((b < 4 ? w[o].x : w[o].y) >> (8 * (b & 3))) * s[o];
+                for (int b = 0; b < 4; b++) {
+                    const uint32_t c = (b < 2 ? w[o].x : w[o].y) >> (16 * (b & 1));
+                    x[o][b] = make_float2((float)(int8_t)c * s[o], (float)(int8_t)(c >> 8) * s[o]);
+                }
         }
         store8(k_out, (size_t)id * 8, F32, x[0]);
         store8(v_out, (size_t)id * 8, F32, x[1]);
@@ -623,40 +608,46 @@ cudaError_t launch_paged_append(const sv_paged& kv, const sv_paged_step& s, cons
     a.head = reinterpret_cast<const int*>(work + l.head);
     a.q_out = r.q_out;
     a.q_out_f32 = r.q_out_type == SV_TYPE_F32;
-    // Heads are split over blocks until there are about four blocks per SM: below that the rows of a page
-    // leave SMs idle, above it the tokens' sines are computed more often than needed.
+    const int rows = kv.page_size < s.max_new ? kv.page_size : s.max_new;    // new rows of one page, at most
+    // Heads are split over blocks until there are about four blocks per SM: fewer leave SMs idle, more compute the
+    // tokens' sines oftener than needed.
     const int want = ceil_div(4 * device_sm_count(), l.page_cap);
     const int groups = want < 1 ? 1 : want > kv.n_kv_head ? kv.n_kv_head : want;
     a.kv_per = ceil_div(kv.n_kv_head, groups);
-    const dim3 grid((unsigned)l.page_cap, (unsigned)ceil_div(kv.n_kv_head, a.kv_per));
-    const int rows = kv.page_size < s.max_new ? kv.page_size : s.max_new;    // new rows of one page, at most
+    a.kv_groups = ceil_div(kv.n_kv_head, a.kv_per);
+    // at least four heads per block: their loads are in flight together
+    a.q_per = ceil_div(s.n_head, want < 1 ? 1 : want) < 4 ? 4 : ceil_div(s.n_head, want < 1 ? 1 : want);
+    const dim3 grid((unsigned)l.page_cap, (unsigned)(rows <= 4 ? a.kv_groups : 2 * a.kv_groups + ceil_div(s.n_head, a.q_per)));
     const int smem = rows * a.n_dims * 4;
     const bool f32 = r.type == SV_TYPE_F32;
-#define SV_TRY(...)                                                                          \
-    {                                                                                        \
-        auto* k32 = __VA_ARGS__;                                                             \
-        if (smem > 40 * 1024) {                                                              \
-            const cudaError_t e = cudaFuncSetAttribute(k32, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); \
-            if (e != cudaSuccess) return e;                                                  \
-        }                                                                                    \
-        return launch_pdl(k32, grid, dim3(threads), (size_t)smem, st, a);                    \
+    const int rot = !r.rope || a.mode == SV_ROPE_NORM ? ROT_OWN : (a.n_dims & 15) == 0 ? ROT_RUN : ROT_ANY;
+    auto launch = [&](auto* kernel, int threads) -> cudaError_t {
+        if (smem > 40 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+            if (e != cudaSuccess) return e;
+        }
+        return launch_pdl(kernel, grid, dim3(threads), (size_t)smem, st, a);
+    };
+#define SV_ROT(NAME, HD_, F_, THREADS_, ...)                                                          \
+    return rot == ROT_OWN   ? launch(NAME<HD_, F_, ROT_OWN, __VA_ARGS__>, THREADS_)                   \
+           : rot == ROT_RUN ? launch(NAME<HD_, F_, ROT_RUN, __VA_ARGS__>, THREADS_)                   \
+                            : launch(NAME<HD_, F_, ROT_ANY, __VA_ARGS__>, THREADS_);
+#define SV_FEW(HD_, NV_)                                                                              \
+    if (kv.head_dim == HD_ && rows <= NV_) {                                                          \
+        if (f32) SV_ROT(paged_append_few, HD_, true, 256, NV_)                                        \
+        else SV_ROT(paged_append_few, HD_, false, 256, NV_)                                           \
     }
-#define SV_FEW(HD_, NV_)                                                                     \
-    if (kv.head_dim == HD_ && rows <= NV_) {                                                 \
-        const int threads = 256;                                                             \
-        if (f32) SV_TRY(paged_append_few<HD_, true, NV_>) else SV_TRY(paged_append_few<HD_, false, NV_>) \
-    }
-#define SV_MANY(HD_, TH_, NV_)                                                               \
-    if (kv.head_dim == HD_ && rows <= NV_ * TH_ * 8 / HD_) {                                 \
-        const int threads = TH_;                                                             \
-        if (f32) SV_TRY(paged_append_many<HD_, true, TH_, NV_>) else SV_TRY(paged_append_many<HD_, false, TH_, NV_>) \
+#define SV_MANY(HD_, TH_, NV_)                                                                        \
+    if (kv.head_dim == HD_ && rows <= NV_ * TH_ * 8 / HD_) {                                          \
+        if (f32) SV_ROT(paged_append_many, HD_, true, TH_, TH_, NV_)                                  \
+        else SV_ROT(paged_append_many, HD_, false, TH_, TH_, NV_)                                     \
     }
     SV_FEW(64, 1) SV_FEW(64, 4) SV_MANY(64, 256, 1) SV_MANY(64, 256, 4)
     SV_FEW(128, 1) SV_FEW(128, 4) SV_MANY(128, 256, 2) SV_MANY(128, 256, 4) SV_MANY(128, 512, 4)
-    SV_FEW(256, 1) SV_FEW(256, 4) SV_MANY(256, 256, 2) SV_MANY(256, 256, 4) SV_MANY(256, 512, 8)
+    SV_FEW(256, 1) SV_FEW(256, 4) SV_MANY(256, 256, 4) SV_MANY(256, 512, 4) SV_MANY(256, 512, 8)
 #undef SV_FEW
 #undef SV_MANY
-#undef SV_TRY
+#undef SV_ROT
     return cudaErrorInvalidValue;
 }
 
