@@ -47,7 +47,7 @@ struct AppendArgs {
     const int4* pages;
     const int* head;
     int kv_per, kv_groups;    // kv heads per block, and blocks for them
-    int q_per;                // query heads per block (many rows)
+    int q_per, q_parts;       // query heads per block, parts of a page's rows (many rows)
     void* q_out;
     bool q_out_f32;
 };
@@ -114,8 +114,18 @@ struct Rotation {
 };
 
 // Where an element's partner is.  ROT_OWN: with the same thread (pairs side by side; no rotation); ROT_RUN: eight
-// elements of another thread (halves of whole runs of eight); ROT_ANY: one by one.
+// elements of another lane (halves of whole runs of eight); ROT_ANY: one by one, from the row again.
 enum : int { ROT_OWN = 0, ROT_RUN = 1, ROT_ANY = 2 };
+
+template <bool F32>
+__device__ __forceinline__ Raw8<F32> from_lane(const Raw8<F32>& r, int src) {
+    Raw8<F32> y;
+#pragma unroll
+    for (int i = 0; i < (F32 ? 2 : 1); i++)
+        y.w[i] = make_uint4(__shfl_sync(0xffffffffu, r.w[i].x, src), __shfl_sync(0xffffffffu, r.w[i].y, src),
+                            __shfl_sync(0xffffffffu, r.w[i].z, src), __shfl_sync(0xffffffffu, r.w[i].w, src));
+    return y;
+}
 
 // cs: the token's cosines [n_dims/2], then its sines.  w: norm weights or null.
 template <int ROT>
@@ -178,15 +188,15 @@ __device__ __forceinline__ float row_norm(const float2* x, float eps) {
     return rsqrtf(t * (1.0f / HD) + eps);          // 2 units of 2^-23
 }
 
-// x = n (x c + x' s), n the row's norm; row points at this thread's first element (partners that are not the
-// thread's own are read from the row again, through L1: pr holds a run of eight)
+// x = n (x c + x' s), n the row's norm.  raw: the thread's eight elements as they came, src: the lane that holds
+// their partners, row: the thread's first element in memory.  Whole warps call it.
 template <int HD, bool F32, int ROT>
-__device__ __forceinline__ void turn_row(const AppendArgs& a, bool normed, const Rotation& r, const Raw8<F32>& pr, const uint8_t* row,
-                                         int e, float2* x) {
+__device__ __forceinline__ void turn_row(const AppendArgs& a, bool normed, const Rotation& r, const Raw8<F32>& raw, int src,
+                                         const uint8_t* row, int e, float2* x) {
     float2 y[4];
     // a dim past n_dims has no partner: 0, not s = 0 times a value that may not be a number
     if constexpr (ROT == ROT_RUN) {
-        to_f32<F32>(pr, y);
+        to_f32<F32>(from_lane<F32>(raw, src), y);
         if (e >= a.n_dims) {
 #pragma unroll
             for (int i = 0; i < 4; i++) y[i] = make_float2(0.0f, 0.0f);
@@ -308,15 +318,14 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
     const int kv0 = blockIdx.y * a.kv_per, kvn = min(a.kv_per, a.kv.n_kv_head - kv0);
     const int units = it.y >= 0 ? 2 * kvn : 0;     // kv head i / 2, K or V; none without a page
     const int q0 = kv0 * a.G, qn = kvn * a.G, q_rows = n * qn;
-    // offset of the partner run (0 where there is none)
-    const int half = a.n_dims >> 1;
-    const int poff = ROT == ROT_RUN && e < a.n_dims ? (e < half ? half : -half) * ES : 0;
+    const int half = a.n_dims >> 1, lane = threadIdx.x & 31;
+    const int partner = ROT == ROT_RUN && e < a.n_dims ? (e < half ? lane + half / 8 : lane - half / 8) : lane;
     // This thread's rows of a pass.  The first pass of both kinds is loaded before the sines are computed.
     const uint8_t* kp = a.k + (size_t)it.x * a.k_nb + (size_t)kv0 * HD * ES + e * ES;
     const uint8_t* vp = a.v + (size_t)it.x * a.v_nb + (size_t)kv0 * HD * ES + e * ES;
     const uint8_t* qp = a.q + (size_t)it.x * a.q_nb + (size_t)q0 * HD * ES + e * ES;
     auto unit_src = [&](int i) { return ((i & 1) == 0 ? kp : vp) + (i >> 1) * (HD * ES); };
-    Raw8<F32> raw[NV], praw[NV], qraw, qpraw;
+    Raw8<F32> raw[NV], qraw;
     float s_old = 0.0f;
     auto load_unit = [&](int i) {
         if (i >= units) return;
@@ -326,10 +335,7 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
         if (it.z > 0) s_old = (is_k ? a.kv.k_scale : a.kv.v_scale)[(size_t)it.y * a.kv.n_kv_head + kv0 + (i >> 1)];
 #pragma unroll
         for (int r = 0; r < NV; r++)
-            if (r < n) {
-                raw[r] = fetch8<F32>(src + r * nb);
-                if (ROT == ROT_RUN && is_k) praw[r] = fetch8<F32>(src + r * nb + poff);
-            }
+            if (r < n) raw[r] = fetch8<F32>(src + r * nb);
     };
     int qr = 0, qh = 0;                            // row and head of this thread's query row
     const uint8_t* qrow = qp;
@@ -339,7 +345,6 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
         if (i >= q_rows) qr = qh = 0;
         qrow = qp + (size_t)qr * a.q_nb + qh * (HD * ES);
         qraw = fetch8<F32>(qrow);
-        if (ROT == ROT_RUN) qpraw = fetch8<F32>(qrow + poff);
     };
     load_unit(u);
     load_q(u);
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
                 for (int j = 0; j < 4; j++) y[j] = x[r][j];
                 Rotation rot;
                 rotation_of<ROT>(a, cs + r * a.n_dims, e, a.kn, &rot);
-                turn_row<HD, F32, ROT>(a, a.kn != nullptr, rot, is_k ? praw[r] : raw[r], is_k ? unit_src(i) + r * a.k_nb : kp, e, y);
+                turn_row<HD, F32, ROT>(a, a.kn != nullptr, rot, raw[r], partner, is_k ? unit_src(i) + r * a.k_nb : kp, e, y);
                 if (is_k) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) x[r][j] = y[j];
@@ -405,7 +410,7 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
         if (a.pairs || a.qn) {
             Rotation rot;
             rotation_of<ROT>(a, cs + qr * a.n_dims, e, a.qn, &rot);
-            turn_row<HD, F32, ROT>(a, a.qn != nullptr, rot, qpraw, qrow, e, x);
+            turn_row<HD, F32, ROT>(a, a.qn != nullptr, rot, qraw, partner, qrow, e, x);
         }
         __syncwarp();                              // q_out may be q: the row's partners have been read
         if (i0 + u < q_rows) store8(a.q_out, ((size_t)(it.x + qr) * a.NH + q0 + qh) * HD + e, a.q_out_f32, x);
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 3 : 2)
     const int e = (threadIdx.x % C) * 8, r0 = threadIdx.x / C;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = a.n_dims >> 1;
-    const int poff = ROT == ROT_RUN && e < a.n_dims ? (e < half ? half : -half) * ES : 0;
+    const int partner = ROT == ROT_RUN && e < a.n_dims ? (e < half ? lane + half / 8 : lane - half / 8) : lane;
     if ((int)blockIdx.y < 2 * a.kv_groups) {
         const bool is_k = (blockIdx.y & 1) == 0;
         const int kv0 = (blockIdx.y >> 1) * a.kv_per, kvn = min(a.kv_per, a.kv.n_kv_head - kv0);
@@ -439,6 +444,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 3 : 2)
         float* scales = (is_k ? a.kv.k_scale : a.kv.v_scale) + (size_t)it.y * a.kv.n_kv_head + kv0;
         uint8_t* pages = static_cast<uint8_t*>(is_k ? a.kv.k : a.kv.v) + ((size_t)it.y * a.kv.n_kv_head + kv0) * a.kv.page_size * HD;
         const bool turned = is_k && (a.pairs || a.kn);
+        // norm weights of the thread's elements and of their partners
+        float2 w[4], wp[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = wp[j] = make_float2(1.0f, 1.0f);
+        if (turned && a.kn) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int d = e + j;
+                const int pd = d >= a.n_dims ? d : a.mode == SV_ROPE_NORM ? d ^ 1 : d < half ? d + half : d - half;
+                const float x = __ldg(a.kn + d), y = __ldg(a.kn + pd);
+                if (j & 1) w[j >> 1].y = x, wp[j >> 1].y = y;
+                else w[j >> 1].x = x, wp[j >> 1].x = y;
+            }
+        }
         Raw8<F32> raw[NV];
         auto load = [&](int hi) {
 #pragma unroll
@@ -463,11 +482,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 3 : 2)
                 if (live) to_f32<F32>(raw[i], x[i]);
                 if (turned) {                      // whole warps go through (the norm's shuffles); a dead row takes the first
                     const uint8_t* row = src + (live ? (size_t)(i * RP) * nb : 0) + hi * (HD * ES);
-                    Raw8<F32> pr;
-                    if (ROT == ROT_RUN) pr = fetch8<F32>(row + poff);
                     Rotation rot;
-                    rotation_of<ROT>(a, cs + (live ? r0 + i * RP : 0) * a.n_dims, e, a.kn, &rot);
-                    turn_row<HD, F32, ROT>(a, a.kn != nullptr, rot, pr, row, e, x[i]);
+                    rotation_of<ROT>(a, cs + (live ? r0 + i * RP : 0) * a.n_dims, e, nullptr, &rot);
+                    if (a.kn) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            rot.c[j] = mul2(rot.c[j], w[j]);
+                            rot.s[j] = mul2(rot.s[j], wp[j]);
+                        }
+                    }
+                    turn_row<HD, F32, ROT>(a, a.kn != nullptr, rot, raw[i], partner, row, e, x[i]);
                 }
                 if (live) watch(x[i], &amax, &bad);
             }
@@ -510,35 +534,39 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 3 : 2)
         return;
     }
     // ---- query rows: a thread keeps its token and chunk, and so its rotation, over the heads
-    constexpr int U = F32 ? 2 : 4;                 // heads whose loads are in flight
-    const int q0 = ((int)blockIdx.y - 2 * a.kv_groups) * a.q_per, qn = min(a.q_per, a.NH - q0);
+    constexpr int U = F32 ? 2 : 4;                 // heads whose loads are in flight while U others are worked on
+    const int y = (int)blockIdx.y - 2 * a.kv_groups, part = y % a.q_parts;
+    const int q0 = y / a.q_parts * a.q_per, qn = min(a.q_per, a.NH - q0);
+    const int rows = (n + a.q_parts - 1) / a.q_parts, first = part * rows, end = min(n, first + rows);
+    if (first >= end) return;
     const bool turned = a.pairs || a.qn;
     if (a.pairs) {
-        fill_turns(a, it.x, n, cs);
+        fill_turns(a, it.x + first, end - first, cs);
         __syncthreads();
     }
-    for (int rb = 0; rb < n; rb += RP) {
-        const bool live = rb + r0 < n;
-        const int r = live ? rb + r0 : 0;
-        Rotation rot;
-        if (turned) rotation_of<ROT>(a, cs + r * a.n_dims, e, a.qn, &rot);
+    for (int rb = first; rb < end; rb += RP) {
+        const bool live = rb + r0 < end;
+        const int r = live ? rb + r0 : first;
         const uint8_t* row = a.q + (size_t)(it.x + r) * a.q_nb + (size_t)q0 * HD * ES + e * ES;
         const size_t to = ((size_t)(it.x + r) * a.NH + q0) * HD + e;
-        for (int hb = 0; hb < qn; hb += U) {
-            Raw8<F32> raw[U], pr[U];
+        Raw8<F32> raw[U], next[U];
 #pragma unroll
-            for (int j = 0; j < U; j++) {
-                const int off = min(hb + j, qn - 1) * (HD * ES);
-                raw[j] = fetch8<F32>(row + off);
-                if (ROT == ROT_RUN) pr[j] = fetch8<F32>(row + off + poff);
+        for (int j = 0; j < U; j++) next[j] = fetch8<F32>(row + min(j, qn - 1) * (HD * ES));
+        Rotation rot;
+        if (turned) rotation_of<ROT>(a, cs + (r - first) * a.n_dims, e, a.qn, &rot);
+        for (int hb = 0; hb < qn; hb += U) {
+#pragma unroll
+            for (int j = 0; j < U; j++) raw[j] = next[j];
+            if (hb + U < qn) {
+#pragma unroll
+                for (int j = 0; j < U; j++) next[j] = fetch8<F32>(row + min(hb + U + j, qn - 1) * (HD * ES));
             }
-            __syncwarp();                          // q_out may be q: these heads' partners have been read
 #pragma unroll
             for (int j = 0; j < U; j++) {
                 float2 x[4];
                 to_f32<F32>(raw[j], x);
-                if (turned) turn_row<HD, F32, ROT>(a, a.qn != nullptr, rot, pr[j], row + min(hb + j, qn - 1) * (HD * ES), e, x);
-                if (ROT == ROT_ANY) __syncwarp();  // as above, for partners that were read one by one
+                if (turned) turn_row<HD, F32, ROT>(a, a.qn != nullptr, rot, raw[j], partner, row + min(hb + j, qn - 1) * (HD * ES), e, x);
+                if (ROT == ROT_ANY) __syncwarp();  // q_out may be q, and partners were read one by one
                 if (live && hb + j < qn) store8(a.q_out, to + (hb + j) * HD, a.q_out_f32, x);
             }
         }
@@ -609,15 +637,18 @@ cudaError_t launch_paged_append(const sv_paged& kv, const sv_paged_step& s, cons
     a.q_out = r.q_out;
     a.q_out_f32 = r.q_out_type == SV_TYPE_F32;
     const int rows = kv.page_size < s.max_new ? kv.page_size : s.max_new;    // new rows of one page, at most
-    // Heads are split over blocks until there are about four blocks per SM: fewer leave SMs idle, more compute the
-    // tokens' sines oftener than needed.
-    const int want = ceil_div(4 * device_sm_count(), l.page_cap);
-    const int groups = want < 1 ? 1 : want > kv.n_kv_head ? kv.n_kv_head : want;
-    a.kv_per = ceil_div(kv.n_kv_head, groups);
+    // Heads (and a page's query rows) are split over blocks until there are about two blocks per SM of each kind:
+    // fewer leave SMs idle, more compute the tokens' sines oftener than needed.
+    const int C = kv.head_dim / 8;
+    const int want = ceil_div(2 * device_sm_count(), l.page_cap);
+    auto at_most = [](int x, int most) { return x < 1 ? 1 : x > most ? most : x; };
+    a.kv_per = ceil_div(kv.n_kv_head, at_most(rows <= 4 ? 2 * want : want, kv.n_kv_head));
     a.kv_groups = ceil_div(kv.n_kv_head, a.kv_per);
-    // at least four heads per block: their loads are in flight together
-    a.q_per = ceil_div(s.n_head, want < 1 ? 1 : want) < 4 ? 4 : ceil_div(s.n_head, want < 1 ? 1 : want);
-    const dim3 grid((unsigned)l.page_cap, (unsigned)(rows <= 4 ? a.kv_groups : 2 * a.kv_groups + ceil_div(s.n_head, a.q_per)));
+    // a block takes at least four heads (their loads are in flight together), and whole passes of rows
+    a.q_per = ceil_div(s.n_head, at_most(want, ceil_div(s.n_head, 4)));
+    const int q_groups = ceil_div(s.n_head, a.q_per);
+    a.q_parts = at_most(ceil_div(want, q_groups), ceil_div(rows, 256 / C));
+    const dim3 grid((unsigned)l.page_cap, (unsigned)(rows <= 4 ? a.kv_groups : 2 * a.kv_groups + q_groups * a.q_parts));
     const int smem = rows * a.n_dims * 4;
     const bool f32 = r.type == SV_TYPE_F32;
     const int rot = !r.rope || a.mode == SV_ROPE_NORM ? ROT_OWN : (a.n_dims & 15) == 0 ? ROT_RUN : ROT_ANY;
