@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 import subprocess
 
 import numpy as np
@@ -98,14 +99,6 @@ class _PagedStep(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ("n_past", "n_new", "table", "q_start", "kv_len", "tok_req", "tok_pos",
                                                "tok_slot", "work")] + \
                [("work_bytes", ctypes.c_size_t), ("err", ctypes.c_void_p)]
-
-
-class _PagedRows(ctypes.Structure):
-    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int),
-                ("q_nb", ctypes.c_size_t), ("k_nb", ctypes.c_size_t), ("v_nb", ctypes.c_size_t),
-                ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
-                ("rope", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
-                ("q_out_type", ctypes.c_int)]
 
 
 class _RopeParams(ctypes.Structure):
@@ -213,7 +206,8 @@ def _torch():
 def _stream(stream):
     if stream is None:
         # the current stream's handle without building a Stream object (3 us a call)
-        return _torch()._C._cuda_getCurrentRawStream(_torch()._C._cuda_getDevice())
+        c = _torch()._C
+        return c._cuda_getCurrentRawStream(c._cuda_getDevice())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -387,28 +381,34 @@ class KvCache:
 
 
 # =================================================================== paged 8-bit cache
+# These calls run once per layer and step, so their Python part is kept to a few microseconds: stride
+# tuples instead of single strides, the row descriptor packed in one call, the stream's raw handle.
+_ROWS = struct.Struct("@PPPiNNNPPfPPPi0P")     # sv_paged_rows
+
+
 def _float_type(fn: str, t) -> int:
     """SV type id of an f16 or f32 tensor."""
-    torch = _torch()
-    if t.dtype == torch.float16:
+    dt = t.dtype
+    if dt is _torch().float16:
         return TYPE_F16
-    if t.dtype == torch.float32:
+    if dt is _torch().float32:
         return TYPE_F32
     raise SvError(fn, -2)
 
 
-def _packed(t, heads: int, hd: int) -> bool:
-    """[T, heads, hd] with a token's heads side by side."""
-    return t.dim() == 3 and t.shape[1] == heads and t.shape[2] == hd and t.stride(2) == 1 and (heads == 1 or t.stride(1) == hd)
+def _row_bytes(t, shape, es: int) -> int:
+    """Bytes from a token's row to the next of t [T, heads, hd] = shape with a token's heads side by side; -1 if it is
+    not laid out so."""
+    if t.shape != shape:
+        return -1
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != shape[2] and shape[1] != 1):
+        return -1
+    return (s0 if shape[0] > 1 else shape[1] * shape[2]) * es
 
 
 def _weights(w, hd: int) -> bool:
-    return w is None or (w.dtype == _torch().float32 and w.is_contiguous() and w.numel() == hd)
-
-
-def _row_bytes(t) -> int:
-    """Bytes from a token's row to the next (one row: its own length)."""
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]) * t.element_size()
+    return w is None or (w.dtype is _torch().float32 and w.is_contiguous() and w.numel() == hd)
 
 
 def _require(fn: str, ok) -> None:
@@ -470,6 +470,7 @@ class PagedStep:
         for name in ("q_start", "kv_len", "tok_req", "tok_pos", "tok_slot", "work", "err"):
             setattr(s, name, getattr(self, name).data_ptr())
         self.n_req, self.n_tokens, self.n_head, self.n_kv_head, self.head_dim = n_req, n_tokens, n_head, n_kv_head, head_dim
+        self._q_shape, self._kv_shape = (n_tokens, n_head, head_dim), (n_tokens, n_kv_head, head_dim)
 
     def plan(self, n_past, n_new, table, free_pages, n_free, stream=None) -> None:
         """Page tables, slot map and work lists of the step (sv_paged_plan): n_past, n_new int32 [n_req],
@@ -510,6 +511,8 @@ class PagedKv:
                           self._scales[i, 1].data_ptr(), n_pages, n_kv_head, page_size, head_dim, self.err.data_ptr())
                    for i in range(n_layer)]
         self._refs = [ctypes.byref(x) for x in self._l]
+        self._rows = (ctypes.c_char * _ROWS.size)()          # sv_paged_rows of the call being made
+        self._rows_ref = ctypes.addressof(self._rows)
 
     def codes(self, layer: int, is_v: bool):
         """torch int8 view [n_pages, n_kv_head, page_size, head_dim] of a layer's K or V codes."""
@@ -525,52 +528,64 @@ class PagedKv:
         k and v [T, n_kv_head, HD], all f16 or all f32, heads packed, any token stride of 16-byte multiples
         (views of one projection's output).  pos: int32 [T] ([4, T] for ROPE_IMROPE), or None: the plan's
         positions.  Returns the rotated queries (f16 unless q_out is given)."""
-        torch = _torch()
-        fn, T = "sv_paged_append", step.n_tokens
+        fn, torch = "sv_paged_append", _torch()
+        dt = q.dtype
+        qt = _float_type(fn, q)
+        es = 2 if qt == TYPE_F16 else 4
+        q_nb, k_nb, v_nb = _row_bytes(q, step._q_shape, es), _row_bytes(k, step._kv_shape, es), _row_bytes(v, step._kv_shape, es)
+        _require(fn, q_nb > 0 and k_nb > 0 and v_nb > 0 and k.dtype is dt and v.dtype is dt)
         if q_out is None:
-            q_out = torch.empty((T, step.n_head, step.head_dim), dtype=torch.float16, device=q.device)
-        hd = self.head_dim
-        _require(fn, q.shape == (T, step.n_head, hd) and k.shape == v.shape == (T, self.n_kv_head, hd) and q_out.shape == q.shape
-                 and q.dtype == k.dtype == v.dtype and q_out.is_contiguous()
-                 and _packed(q, step.n_head, hd) and _packed(k, self.n_kv_head, hd) and _packed(v, self.n_kv_head, hd)
-                 and (pos is None or (pos.dtype == torch.int32 and pos.is_contiguous()
-                                      and pos.numel() == (4 * T if rope is not None and rope.mode == ROPE_IMROPE else T)))
-                 and _weights(q_norm, hd) and _weights(k_norm, hd))
-        r = _PagedRows(q.data_ptr(), k.data_ptr(), v.data_ptr(), _float_type(fn, q), _row_bytes(q), _row_bytes(k),
-                       _row_bytes(v), _ptr(q_norm), _ptr(k_norm), eps, None if rope is None else rope.h, _ptr(pos),
-                       q_out.data_ptr(), _float_type(fn, q_out))
-        _check(fn, _lib.sv_paged_append(self._refs[layer], step._ref, ctypes.byref(r), _stream(stream)))
+            q_out = torch.empty_like(q, dtype=torch.float16, memory_format=torch.contiguous_format)
+            ot = TYPE_F16
+        else:
+            ot = _float_type(fn, q_out)
+            _require(fn, q_out.shape == step._q_shape and q_out.is_contiguous())
+        if q_norm is not None or k_norm is not None:
+            _require(fn, _weights(q_norm, self.head_dim) and _weights(k_norm, self.head_dim))
+        _require(fn, rope is None or rope.h)
+        if pos is not None:
+            n = step.n_tokens * (4 if rope is not None and rope.mode == ROPE_IMROPE else 1)
+            _require(fn, pos.dtype is torch.int32 and pos.is_contiguous() and pos.numel() == n)
+        _ROWS.pack_into(self._rows, 0, q.data_ptr(), k.data_ptr(), v.data_ptr(), qt, q_nb, k_nb, v_nb,
+                        0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), eps,
+                        0 if rope is None else rope.h, 0 if pos is None else pos.data_ptr(), q_out.data_ptr(), ot)
+        _check(fn, _lib.sv_paged_append(self._refs[layer], step._ref, self._rows_ref, _stream(stream)))
         return q_out
 
     def read(self, layer: int, slots, k_out=None, v_out=None, stream=None):
         """Rows of the cache as numbers (sv_paged_read): slots int32 [n] (page * page_size + offset) ->
         k, v [n, n_kv_head, head_dim], f16 unless outputs are given."""
-        torch = _torch()
-        fn = "sv_paged_read"
+        fn, torch = "sv_paged_read", _torch()
         shape = (slots.numel(), self.n_kv_head, self.head_dim)
         if k_out is None:
-            k_out = torch.empty(shape, dtype=torch.float16, device=slots.device)
+            k_out = slots.new_empty(shape, dtype=torch.float16)
+        else:
+            _require(fn, k_out.shape == shape and k_out.is_contiguous())
         if v_out is None:
-            v_out = torch.empty(shape, dtype=k_out.dtype, device=slots.device)
-        _require(fn, slots.dtype == torch.int32 and slots.is_contiguous() and k_out.shape == v_out.shape == shape
-                 and k_out.dtype == v_out.dtype and k_out.is_contiguous() and v_out.is_contiguous())
+            v_out = torch.empty_like(k_out)
+        else:
+            _require(fn, v_out.shape == shape and v_out.is_contiguous() and k_out.dtype is v_out.dtype)
+        _require(fn, slots.dtype is torch.int32 and slots.is_contiguous())
         _check(fn, _lib.sv_paged_read(self._refs[layer], slots.data_ptr(), shape[0], k_out.data_ptr(), v_out.data_ptr(),
-                                       _float_type(fn, k_out), _stream(stream)))
+                                     _float_type(fn, k_out), _stream(stream)))
         return k_out, v_out
 
     def attn(self, layer: int, step: PagedStep, q, scale: float, window: int = 0, out=None, stream=None):
         """Causal attention of the step's rows q [T, n_head, HD] (f16/f32, heads packed) over the pages
         (sv_paged_attn); window > 0: the last `window` positions only.  Returns [T, n_head, HD] f16 unless
         out is given."""
-        torch = _torch()
-        fn = "sv_paged_attn"
+        fn, torch = "sv_paged_attn", _torch()
+        qt = _float_type(fn, q)
+        q_nb = _row_bytes(q, step._q_shape, 2 if qt == TYPE_F16 else 4)
+        _require(fn, q_nb > 0)
         if out is None:
-            out = torch.empty((step.n_tokens, step.n_head, step.head_dim), dtype=torch.float16, device=q.device)
-        _require(fn, q.shape == out.shape == (step.n_tokens, step.n_head, self.head_dim)
-                 and _packed(q, step.n_head, self.head_dim) and out.is_contiguous())
-        _check(fn, _lib.sv_paged_attn(self._refs[layer], step._ref, q.data_ptr(), _float_type(fn, q),
-                                       _row_bytes(q), scale, window, out.data_ptr(),
-                                       _float_type(fn, out), _stream(stream)))
+            out = torch.empty_like(q, dtype=torch.float16, memory_format=torch.contiguous_format)
+            ot = TYPE_F16
+        else:
+            ot = _float_type(fn, out)
+            _require(fn, out.shape == step._q_shape and out.is_contiguous())
+        _check(fn, _lib.sv_paged_attn(self._refs[layer], step._ref, q.data_ptr(), qt, q_nb, scale, window, out.data_ptr(), ot,
+                                     _stream(stream)))
         return out
 
     def release(self, table, req, kv_len, free_pages, n_free, stream=None) -> None:
