@@ -7,7 +7,8 @@
 //   head      counts of the lists below
 //   req       int4 per request: first row, rows, tokens held before, tokens held after
 //   page      int4 per page that the step writes to: first row, page, first offset, rows
-//   dec       int2 per decode item: request, split | splits << 16
+//   dec       two int4 per decode segment: request, its tiles [a, b), split | splits << 16; its req entry
+//   cta       first segment of each decode CTA (and one past the last)
 //   pre       int4 per prefill item: request, query tile, split, splits
 //   tickets   arrival counters of the split merges (zeroed by the plan, and again by each merge)
 //   *_part    unnormalised outputs of the splits; *_ml their running maximum and sum
@@ -26,21 +27,21 @@ constexpr int kDecRows = 16;      // most query rows of one decode unit
 // a prefill kernel runs beside it anyway, else the sixteen-row one (one decode launch either way).
 inline int few_rows(int64_t most_rows) { return most_rows <= 8 || most_rows > kDecRows ? 8 : kDecRows; }
 constexpr int kDecTile = 64;      // keys per decode tile
-// decode CTAs that one SM holds (shared memory: a ring of K and V tiles each)
-constexpr int dec_ctas_per_sm(int hd) { return hd == 256 ? 2 : 3; }
+// decode CTAs that one SM holds (shared memory: a ring of K and V tiles each; registers: the sixteen-row kernel's outputs)
+constexpr int dec_ctas_per_sm(int hd, bool sixteen) { return (hd == 256 ? 2 : 3) - (sixteen ? 1 : 0); }
 constexpr int pre_rows(int hd) { return hd == 256 ? 128 : 256; }   // query rows of one prefill unit
 constexpr int pre_tile(int hd) { return hd == 256 ? 64 : 128; }    // keys per prefill tile
 // a split shorter than this costs more in its start and merge than it saves
-constexpr int kDecMinTiles = 2;
+constexpr int kDecMinTiles = 4;
 constexpr int kPreMinTiles = 4;
 
-enum : int { PH_PAGES = 0, PH_DEC = 1, PH_PRE = 2 };
+enum : int { PH_PAGES = 0, PH_PRE = 1 };
 
 struct StepLayout {
     int page_cap = 0, dec_cap = 0, pre_cap = 0;     // most entries of each list
     int few = kDecRows;                             // rows of a decode unit, at most
-    int dec_slots = 1, pre_slots = 1;               // items that run at once, per kv head
-    size_t head = 0, req = 0, page = 0, dec = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
+    int dec_slots = 1, pre_slots = 1;               // CTAs that run at once, per kv head
+    size_t head = 0, req = 0, page = 0, dec = 0, cta = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
     size_t bytes = 0;
     int n_ticks = 0;
 };

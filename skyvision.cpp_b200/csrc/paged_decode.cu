@@ -1,7 +1,9 @@
 // paged_decode.cu - attention of requests with few rows over the paged 8-bit cache.
 //
-// One CTA works on one item of the plan: (request, kv head, a piece of its keys).  The request's rows
-// (new tokens x query heads of the kv head, at most 16) all use every key that is loaded:
+// The key tiles of all requests form one line per kv head, cut into equal pieces, one CTA each, as many as
+// run at once: no second wave, no CTA with more to do than another, whatever the lengths.  A CTA's part of a request
+// is a segment.  The request's rows (new tokens x query heads of the kv head, at most 16) all use every key
+// that is loaded:
 //   s_rj = scale log2(e) ks[page(j)] (q_r . c_j),   p_rj = exp2(s_rj - m_r),
 //   o_r  = sum_j p_rj vs[page(j)] c'_j / sum_j p_rj
 // A scale belongs to a page and head, so it multiplies finished dot products: codes enter the tensor
@@ -21,8 +23,8 @@
 // a vote, so a tile normally needs no shuffle and no rescaling; p <= 2^8 is far inside f16.  P is rounded to f16
 // for the second product (2^-12 relative on average, like the f16 output itself); sums stay f32.  P also
 // carries vs / v_ref, where v_ref trails the largest vs seen by at most 4.
-// Pieces of one request and head meet in the work space; the last to arrive (a ticket) adds them in order,
-// so results do not depend on which one that is.
+// The warps of a CTA meet pairwise in shared memory.  Segments of one request and head meet in the work space; the
+// last to arrive (a ticket) adds them in order, so results do not depend on which one that is.
 //
 // Bound: HBM, 2 HD + 8 / page_size bytes per key and kv head.
 #include "common.cuh"
@@ -36,20 +38,21 @@ constexpr int kWarps = 4;                       // consumers
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr float kLazyLog2 = 8.0f;
 
-template <int HD>
+template <int HD, int NT>
 struct DecCfg {
     static constexpr int COLS = HD < 128 ? HD : 128;          // bytes of one box row
     static constexpr int SLABS = HD / COLS;
     static constexpr int PART = kDecTile * HD;                // K or V codes of a tile
     static constexpr int STAGE = 2 * PART;
     static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 4 : 3;
-    static constexpr int OFF_SC = STAGES * STAGE;             // float2 [STAGES][4]: K and V scale of each group
+    static constexpr int PITCH = HD + 4;                      // floats per row of a partial output
+    static constexpr int BUFS = HD == 256 ? 1 : 2;            // warps whose partial outputs fit at once
+    static constexpr int OFF_PART = STAGES * STAGE;           // float [BUFS][8 NT][PITCH]
+    static constexpr int OFF_SC = OFF_PART + BUFS * 8 * NT * PITCH * 4;   // float2 [STAGES][4]: each group's K and V scale
     static constexpr int OFF_OK = OFF_SC + STAGES * 32;       // int [STAGES][4]: the group's page exists
     static constexpr int OFF_BAR = OFF_OK + STAGES * 16;
-    static constexpr int OFF_ML = OFF_BAR + STAGES * 16;      // float [3][kWarps][16]
-    static constexpr int SMEM = OFF_ML + 3 * kWarps * 16 * 4 + 16;
-    static constexpr int PITCH = HD + 4;                      // floats per row of the warps' partial outputs
-    static_assert(kWarps * kDecRows * PITCH * 4 <= OFF_SC, "the warps' partials reuse the ring");
+    static constexpr int OFF_ML = OFF_BAR + STAGES * 16;      // float2 [kWarps][16]: maximum and sum, then int: last
+    static constexpr int SMEM = OFF_ML + kWarps * 16 * 8 + 16;
 };
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -78,24 +81,48 @@ __device__ __forceinline__ uint32_t col16(uint32_t r, uint32_t c) {
     return COLS == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
+// A segment: requests's tiles [j0, j1) of 64 keys, split of ns.
+struct Seg {
+    int req, split, ns, j0, j1;
+    int4 rq;                     // first row, rows, keys held before, after
+};
+
+__device__ __forceinline__ Seg seg_of(const PagedAttn& a, int i) {
+    const int4* d = reinterpret_cast<const int4*>(a.work + a.l.dec) + 2 * (size_t)i;
+    const int4 x = __ldg(d);
+    Seg s;
+    s.rq = __ldg(d + 1);
+    s.req = x.x;
+    s.split = x.w & 0xffff;
+    s.ns = x.w >> 16;
+    // the plan cut all of the request's tiles; a window leaves fewer, shared in the same proportion
+    const int planned = (s.rq.z + s.rq.y + kDecTile - 1) / kDecTile;
+    const int lo = a.window > 0 ? max(0, s.rq.z - a.window + 1) / kDecTile : 0;
+    const int n = max(0, (s.rq.w + kDecTile - 1) / kDecTile - lo);
+    s.j0 = lo + (n == planned ? x.y : (int)((long long)n * x.y / planned));
+    s.j1 = lo + (n == planned ? x.z : (int)((long long)n * x.z / planned));
+    return s;
+}
+
 // NT: row tiles of 8
 template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? dec_ctas_per_sm(HD) : dec_ctas_per_sm(HD) - 1)
+__global__ void __launch_bounds__(kThreads, dec_ctas_per_sm(HD, NT == 2))
 paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                     const __grid_constant__ PagedAttn a) {
-    using C = DecCfg<HD>;
+    using C = DecCfg<HD, NT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* part = reinterpret_cast<float*>(smem + C::OFF_PART);
     float2* sc = reinterpret_cast<float2*>(smem + C::OFF_SC);
     int* okp = reinterpret_cast<int*>(smem + C::OFF_OK);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* empty = full + C::STAGES;
-    float* s_ml = reinterpret_cast<float*>(smem + C::OFF_ML);
-    int* s_last = reinterpret_cast<int*>(s_ml + 3 * kWarps * 16);
+    float2* s_ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
+    int* s_last = reinterpret_cast<int*>(s_ml + kWarps * 16);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int NKV = a.kv.n_kv_head;
-    const int h = blockIdx.x % NKV, item = blockIdx.x / NKV;
+    const int h = blockIdx.x % NKV, cta = blockIdx.x / NKV;
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
             mbar_init(&full[s], 1);
@@ -110,77 +137,103 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     __syncthreads();
     pdl_wait();
     if (threadIdx.x == 0) pdl_trigger();
-    const int n_items = reinterpret_cast<const int*>(a.work + a.l.head)[PH_DEC];
-    if (item >= n_items) return;
-    const int2 it = reinterpret_cast<const int2*>(a.work + a.l.dec)[item];
-    const int split = it.y & 0xffff, ns = it.y >> 16;
-    const int4 rq = reinterpret_cast<const int4*>(a.work + a.l.req)[it.x];   // first row, rows, held before, after
-    const int rows = rq.y * a.G;
-    const int lo_key = a.window > 0 ? max(0, rq.z - a.window + 1) : 0;
-    const int t_lo = lo_key / kDecTile, t_hi = (rq.w + kDecTile - 1) / kDecTile;
-    const int nt_all = max(0, t_hi - t_lo);
-    const int j0 = t_lo + (int)((long long)nt_all * split / ns), j1 = t_lo + (int)((long long)nt_all * (split + 1) / ns);
-    const int n = j1 - j0;
+    const int* first_seg = reinterpret_cast<const int*>(a.work + a.l.cta) + cta;
+    const int g0 = __ldg(first_seg), g1 = __ldg(first_seg + 1);
 
     if (warp == kWarps) {
-        // ================= producer: lane g holds group j0 * 4 + (batch of 32) + g's page and scales
+        // ================= producer: lane l holds the page and scales of group 4 j0 + (batch of 32) + l
         const int lg = 31 - __clz(a.kv.page_size);
-        const int g_end = (rq.w + 15) >> 4;                       // groups that hold a key
-        const int32_t* row = a.table + (size_t)it.x * a.max_blocks;
-        auto page_of = [&](int g) { return g < min(g_end, 4 * j1) ? __ldg(row + ((g << 4) >> lg)) : 0; };
-        auto valid = [&](int g, int p) { return g < g_end && p >= 0 && p < a.kv.n_pages; };
-        int p0 = page_of(4 * j0 + lane);
-        int p1 = page_of(4 * j0 + 32 + lane);
-        float2 s0 = make_float2(0.0f, 0.0f);
-        bool v0 = valid(4 * j0 + lane, p0);
-        auto scales = [&](int p, bool v) {
-            float2 s = make_float2(0.0f, 0.0f);
-            if (v) {
-                s.x = __ldg(a.kv.k_scale + (size_t)p * NKV + h);
-                s.y = __ldg(a.kv.v_scale + (size_t)p * NKV + h);
-            }
-            return s;
+        struct Batch {
+            int page;
+            bool ok;
+            float2 s;
         };
-        s0 = scales(p0, v0);
-        float2 s1 = scales(p1, valid(4 * j0 + 32 + lane, p1));
-        for (int i = 0; i < n; i++) {
-            const int st = i % C::STAGES, at = (4 * i) & 31;
-            if (i > 0 && at == 0) {                               // the next 32 groups, looked up 8 tiles ago
-                p0 = p1;
-                s0 = s1;
-                const int g = 4 * (j0 + i) + 32 + lane;
-                v0 = valid(g - 32, p0);
-                p1 = page_of(g);
-                s1 = scales(p1, valid(g, p1));
+        auto page_of = [&](const Seg& s, int g) {
+            return g < min((s.rq.w + 15) >> 4, 4 * s.j1) ? __ldg(a.table + (size_t)s.req * a.max_blocks + ((g << 4) >> lg)) : -1;
+        };
+        auto batch_of = [&](int p) {
+            Batch b;
+            b.page = p;
+            b.ok = p >= 0 && p < a.kv.n_pages;
+            b.s = make_float2(0.0f, 0.0f);
+            if (b.ok) {
+                b.s.x = __ldg(a.kv.k_scale + (size_t)p * NKV + h);
+                b.s.y = __ldg(a.kv.v_scale + (size_t)p * NKV + h);
             }
-            bool ok = true;
-            if (lane == 0 && i >= C::STAGES) ok = mbar_wait(&empty[st], ((i / C::STAGES) + 1) & 1, a.err);
-            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-            const int src = at + (lane & 3);
-            const int page = __shfl_sync(0xffffffffu, p0, src);
-            const bool v = __shfl_sync(0xffffffffu, (int)v0, src) != 0;
-            const float2 s = make_float2(__shfl_sync(0xffffffffu, s0.x, src), __shfl_sync(0xffffffffu, s0.y, src));
-            const int grp = 4 * (j0 + i) + (lane & 3);
-            if (lane < 4) {
-                sc[st * 4 + lane] = make_float2(s.x * a.scale_log2, s.y);
-                okp[st * 4 + lane] = v;
-                if (!v && grp < g_end && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
-            }
-            const unsigned have = __ballot_sync(0xffffffffu, v && lane < 4);
-            if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * 16 * HD * 2));
-            __syncwarp();
-            if (v && lane < 8 * C::SLABS) {
-                const bool is_v = (lane & 4) != 0;
-                const int slab = lane >> 3;
-                const int y = ((page * NKV + h) << lg) + ((grp << 4) & (a.kv.page_size - 1));
-                uint8_t* dst = smem + st * C::STAGE + (is_v ? C::PART : 0) + slab * (kDecTile * C::COLS) + (lane & 3) * 16 * C::COLS;
-                tma_load_2d(dst, is_v ? &tmv : &tmk, slab * C::COLS, y, &full[st]);
-            }
+            return b;
+        };
+        int tile = 0;                                             // of the ring, over all segments
+        bool ok = true;
+        Seg s;
+        int p1 = -1;
+        Batch b0, b1;
+        if (g0 < g1) {
+            s = seg_of(a, g0);
+            b0 = batch_of(page_of(s, 4 * s.j0 + lane));
+            p1 = page_of(s, 4 * s.j0 + 32 + lane);
         }
-        // the ring becomes the warps' scratch below: every load has landed, since every tile was waited for
-    } else {
-        // ================= consumers
-        const int gq = lane >> 2, tq = lane & 3;
+        for (int g = g0; g < g1 && ok; g++) {
+            const int n = s.j1 - s.j0;
+            Seg nx = s;
+            Batch nb = b0;
+            int np = -1;
+            b1 = batch_of(p1);
+            for (int i = 0; i < n; i++, tile++) {
+                const int st = tile % C::STAGES, at = (4 * i) & 31;
+                if (i > 0 && at == 0) {                           // the next 32 groups, looked up 8 tiles ago
+                    b0 = b1;
+                    b1 = batch_of(page_of(s, 4 * (s.j0 + i) + 32 + lane));
+                }
+                if (lane == 0 && tile >= C::STAGES) ok = mbar_wait(&empty[st], ((tile / C::STAGES) + 1) & 1, a.err);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (!ok) break;
+                const int src = at + (lane & 3);
+                const int page = __shfl_sync(0xffffffffu, b0.page, src);
+                const bool v = __shfl_sync(0xffffffffu, (int)b0.ok, src) != 0;
+                const float2 x = make_float2(__shfl_sync(0xffffffffu, b0.s.x, src), __shfl_sync(0xffffffffu, b0.s.y, src));
+                const int grp = 4 * (s.j0 + i) + (lane & 3);
+                if (lane < 4) {
+                    sc[st * 4 + lane] = make_float2(x.x * a.scale_log2, x.y);
+                    okp[st * 4 + lane] = v;
+                    if (!v && grp * 16 < s.rq.w && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
+                }
+                const unsigned have = __ballot_sync(0xffffffffu, v && lane < 4);
+                if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(__popc(have) * 16 * HD * 2));
+                __syncwarp();
+                if (v && lane < 8 * C::SLABS) {
+                    const bool is_v = (lane & 4) != 0;
+                    const int slab = lane >> 3;
+                    const int y = ((page * NKV + h) << lg) + ((grp << 4) & (a.kv.page_size - 1));
+                    uint8_t* dst = smem + st * C::STAGE + (is_v ? C::PART : 0) + slab * (kDecTile * C::COLS) + (lane & 3) * 16 * C::COLS;
+                    tma_load_2d(dst, is_v ? &tmv : &tmk, slab * C::COLS, y, &full[st]);
+                }
+                // the next segment's lookups, once this one's first tiles are on their way
+                if (g + 1 < g1 && i == min(n, C::STAGES) - 1) {
+                    nx = seg_of(a, g + 1);
+                    nb = batch_of(page_of(nx, 4 * nx.j0 + lane));
+                    np = page_of(nx, 4 * nx.j0 + 32 + lane);
+                }
+            }
+            if (n == 0 && g + 1 < g1) {
+                nx = seg_of(a, g + 1);
+                nb = batch_of(page_of(nx, 4 * nx.j0 + lane));
+                np = page_of(nx, 4 * nx.j0 + 32 + lane);
+            }
+            s = nx;
+            b0 = nb;
+            p1 = np;
+        }
+        return;
+    }
+    // ================= consumers
+    const int gq = lane >> 2, tq = lane & 3;
+    const int k0 = gq & 1 ? gq ^ 4 : gq;                       // key of MMA index gq
+    const int c0 = 2 * tq, c1 = (2 * tq + 1) ^ 4;              // keys of MMA indexes 2 tq, 2 tq + 1
+    int tile = 0;
+    for (int sg = g0; sg < g1; sg++) {
+        const Seg sgm = seg_of(a, sg);
+        const int4 rq = sgm.rq;
+        const int rows = rq.y * a.G, n = sgm.j1 - sgm.j0;
         // Q^T fragments: row gq (of each row tile), bytes 16 tq.. of each 64-dim group over four k-steps
         uint32_t qf[NT][HD / 64][8];
 #pragma unroll
@@ -212,19 +265,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 }
             }
         }
-        // this thread's columns: rows 8 r + 2 tq + {0, 1}; keys they see: [lo, hi)
-        int lo[NT][2], hi[NT][2];
-        int lo_max = 0, hi_min = INT32_MAX;
-#pragma unroll
-        for (int r = 0; r < NT; r++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int pos = rq.z + min(8 * r + 2 * tq + e, rows - 1) / a.G;
-                lo[r][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-                hi[r][e] = min(pos + 1, rq.w);
-                lo_max = max(lo_max, lo[r][e]);
-                hi_min = min(hi_min, hi[r][e]);
-            }
+        // Keys that every row of the segment sees: [lo_all, hi_all); only tiles outside need the mask
+        const int pos1 = rq.z + rq.y - 1;
+        const int lo_all = a.window > 0 ? max(0, pos1 - a.window + 1) : 0, hi_all = min(rq.z + 1, rq.w);
         float o[HD / 16][NT][4];
 #pragma unroll
         for (int m = 0; m < HD / 16; m++)
@@ -235,17 +278,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         float mref[NT][2], l[NT][2], vref = 0.0f, vinv = 0.0f;
 #pragma unroll
         for (int r = 0; r < NT; r++) mref[r][0] = mref[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
-        const int k0 = gq & 1 ? gq ^ 4 : gq;                       // key of MMA index gq
-        const int c0 = 2 * tq, c1 = (2 * tq + 1) ^ 4;              // keys of MMA indexes 2 tq, 2 tq + 1
 
-        for (int i = 0; i < n; i++) {
-            const int st = i % C::STAGES;
-            const bool got = mbar_wait(&full[st], (i / C::STAGES) & 1, a.err);
-            if (!__all_sync(0xffffffffu, got)) break;
-            const int kb = (j0 + i) * kDecTile + 16 * warp;        // first key of this warp's group
+        for (int i = 0; i < n; i++, tile++) {
+            const int st = tile % C::STAGES;
+            const bool got = mbar_wait(&full[st], (tile / C::STAGES) & 1, a.err);
+            if (!__all_sync(0xffffffffu, got)) return;             // the error bit is set; nothing can be trusted
+            const int kb = (sgm.j0 + i) * kDecTile + 16 * warp;    // first key of this warp's group
             const float2 s2 = sc[st * 4 + warp];
             const bool there = okp[st * 4 + warp] != 0;
-            if (there && kb < rq.w) {
+            if (there) {
                 const uint8_t* kt = smem + st * C::STAGE;
                 const uint8_t* vt = kt + C::PART;
                 float s[NT][4];
@@ -274,13 +315,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 for (int r = 0; r < NT; r++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) s[r][e] *= s2.x;
-                if (kb < lo_max || kb + 16 > hi_min) {
+                if (kb < lo_all || kb + 16 > hi_all) {
 #pragma unroll
                     for (int r = 0; r < NT; r++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int key = kb + k0 + (e >> 1) * 8;
-                            if (key < lo[r][e & 1] || key >= hi[r][e & 1]) s[r][e] = -INFINITY;
+                            const int pos = rq.z + min(8 * r + 2 * tq + (e & 1), rows - 1) / a.G;
+                            if (key >= min(pos + 1, rq.w) || (a.window > 0 && key < pos - a.window + 1)) s[r][e] = -INFINITY;
                         }
                 }
 #pragma unroll
@@ -364,128 +406,162 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
         }
-        // ---- this warp's partial: row sums over the quads' lanes, outputs in v_ref units
+        // ---- one partial of the CTA: the warps' maxima and sums, then outputs added (3, 2 into 1, 0, then 1 into 0; one
+        // after the other with one buffer)
 #pragma unroll
         for (int r = 0; r < NT; r++)
 #pragma unroll
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], w);
-        asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");   // every consumer is past the ring
-        float* part = reinterpret_cast<float*>(smem) + warp * kDecRows * C::PITCH;
-        constexpr int VB = HD >= 128 ? 16 : 8;
-#pragma unroll
-        for (int m = 0; m < HD / 16; m++) {
-            const int d = (m / (VB / 2)) * 128 + VB * gq + 2 * (m % (VB / 2));
-#pragma unroll
-            for (int r = 0; r < NT; r++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                    *reinterpret_cast<float2*>(part + (8 * r + 2 * tq + e) * C::PITCH + d) =
-                        make_float2(o[m][r][e] * vref, o[m][r][e + 2] * vref);
-        }
+        asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");   // the scratch's last readers are done
         if (gq == 0) {
 #pragma unroll
             for (int r = 0; r < NT; r++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    s_ml[warp * 16 + 8 * r + 2 * tq + e] = mref[r][e];
-                    s_ml[(kWarps + warp) * 16 + 8 * r + 2 * tq + e] = l[r][e];
+                for (int e = 0; e < 2; e++) s_ml[warp * 16 + 8 * r + 2 * tq + e] = make_float2(mref[r][e], l[r][e]);
+        }
+        asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+        constexpr int VB = HD >= 128 ? 16 : 8;
+        auto dim_of = [&](int m) { return (m / (VB / 2)) * 128 + VB * gq + 2 * (m % (VB / 2)); };
+#pragma unroll
+        for (int r = 0; r < NT; r++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w * 16 + 8 * r + 2 * tq + e].x);
+                const float f = mref[r][e] == -INFINITY ? 0.0f : vref * fast_exp2(mref[r][e] - M);
+#pragma unroll
+                for (int m = 0; m < HD / 16; m++) {
+                    o[m][r][e] *= f;
+                    o[m][r][e + 2] *= f;
                 }
-        }
-    }
-    __syncthreads();
-    // ---- the warps' partials of each row become one
-    const int unit = item * NKV + h, first = (item - split) * NKV + h;
-    float* wo = reinterpret_cast<float*>(a.work + a.l.dec_part) + (size_t)unit * kDecRows * HD;
-    float2* wml = reinterpret_cast<float2*>(a.work + a.l.dec_ml) + (size_t)unit * kDecRows;
-    auto store = [&](int r, int d, float4 x) {
-        const size_t at = ((size_t)(rq.x + r / a.G) * a.n_head + h * a.G + r % a.G) * HD + d;
-        if (a.out_type == SV_TYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = x;
-        else *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at) = make_uint2(pack_h2(x.x, x.y), pack_h2(x.z, x.w));
-    };
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
-        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        float M = -INFINITY, L = 0.0f;
+            }
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w * 16 + r]);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int step = C::BUFS == 2 ? 2 : 3; step > 0; step = C::BUFS == 2 ? step >> 1 : step - 1) {
+            const int slot = C::BUFS == 2 ? (warp & (step - 1)) : 0;
+            const bool gives = C::BUFS == 2 ? warp >= step && warp < 2 * step : warp == step;
+            const bool takes = C::BUFS == 2 ? warp < step : warp == step - 1;
+            if (gives) {
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            const float m = s_ml[w * 16 + r], f = m == -INFINITY ? 0.0f : fast_exp2(m - M);
-            const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) + (w * kDecRows + r) * C::PITCH + d);
-            L = fmaf(f, s_ml[(kWarps + w) * 16 + r], L);
-            x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+                for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+                    for (int r = 0; r < NT; r++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            *reinterpret_cast<float2*>(part + (slot * 8 * NT + 8 * r + 2 * tq + e) * C::PITCH + dim_of(m)) =
+                                make_float2(o[m][r][e], o[m][r][e + 2]);
+            }
+            asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+            if (takes) {
+#pragma unroll
+                for (int m = 0; m < HD / 16; m++)
+#pragma unroll
+                    for (int r = 0; r < NT; r++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float2* p = reinterpret_cast<float2*>(part + (slot * 8 * NT + 8 * r + 2 * tq + e) * C::PITCH + dim_of(m));
+                            const float2 x = *p;
+                            o[m][r][e] += x.x;
+                            o[m][r][e + 2] += x.y;
+                            if (step == 1) *p = make_float2(o[m][r][e], o[m][r][e + 2]);
+                        }
+            }
+            asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
         }
-        if (ns == 1) {
+        // ---- row r of the CTA's partial is now part[r]; its maximum and sum
+        const int ns = sgm.ns;
+        const int unit = sg * NKV + h, first = (sg - sgm.split) * NKV + h;
+        float* wo = reinterpret_cast<float*>(a.work + a.l.dec_part) + (size_t)unit * kDecRows * HD;
+        float2* wml = reinterpret_cast<float2*>(a.work + a.l.dec_ml) + (size_t)unit * kDecRows;
+        auto store = [&](int r, int d, float4 x) {
+            const size_t at = ((size_t)(rq.x + r / a.G) * a.n_head + h * a.G + r % a.G) * HD + d;
+            if (a.out_type == SV_TYPE_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = x;
+            else *reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at) = make_uint2(pack_h2(x.x, x.y), pack_h2(x.z, x.w));
+        };
+        for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) {
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w * 16 + r].x);
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                const float2 x = s_ml[w * 16 + r];
+                L = fmaf(x.x == -INFINITY ? 0.0f : fast_exp2(x.x - M), x.y, L);
+            }
+            const float4 x = *reinterpret_cast<const float4*>(part + r * C::PITCH + d);
+            if (ns == 1) {
+                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+                store(r, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+            } else {
+                *reinterpret_cast<float4*>(wo + (size_t)r * HD + d) = x;
+                if (d == 0) wml[r] = make_float2(M, L);
+            }
+        }
+        if (ns == 1) continue;
+        // ---- segments of one request and head: the last to arrive adds them, in order
+        __threadfence();
+        asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+        if (threadIdx.x == 0) {
+            int* ticket = reinterpret_cast<int*>(a.work + a.l.tick) + first;
+            const int last = atomicAdd(ticket, 1) == ns - 1;
+            if (last) *ticket = 0;                                     // ready for the next layer
+            *s_last = last;
+        }
+        asm volatile("barrier.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+        if (!*s_last) continue;
+        __threadfence();
+        const float* po = reinterpret_cast<const float*>(a.work + a.l.dec_part) + (size_t)first * kDecRows * HD;
+        const float2* pml = reinterpret_cast<const float2*>(a.work + a.l.dec_ml) + (size_t)first * kDecRows;
+        const size_t so = (size_t)NKV * kDecRows * HD, sm = (size_t)NKV * kDecRows;
+        for (int i = threadIdx.x; i < rows * (HD / 4); i += kWarps * 32) {
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            float M = -INFINITY, L = 0.0f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s0 = 0; s0 < ns; s0 += 8) {                       // eight segments' loads in flight
+                float2 ml[8];
+                float4 y[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const int s = min(s0 + u, ns - 1);
+                    ml[u] = __ldcg(pml + s * sm + r);
+                    y[u] = __ldcg(reinterpret_cast<const float4*>(po + s * so + (size_t)r * HD + d));
+                }
+                float mn = M;
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    if (s0 + u >= ns) ml[u] = make_float2(-INFINITY, 0.0f);
+                    mn = fmaxf(mn, ml[u].x);
+                }
+                if (mn == -INFINITY) continue;
+                const float g = M == -INFINITY ? 0.0f : fast_exp2(M - mn);
+                M = mn;
+                L *= g;
+                x.x *= g; x.y *= g; x.z *= g; x.w *= g;
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const float f = ml[u].x == -INFINITY ? 0.0f : fast_exp2(ml[u].x - mn);
+                    L = fmaf(f, ml[u].y, L);
+                    x.x = fmaf(f, y[u].x, x.x); x.y = fmaf(f, y[u].y, x.y); x.z = fmaf(f, y[u].z, x.z); x.w = fmaf(f, y[u].w, x.w);
+                }
+            }
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
             store(r, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-        } else {
-            *reinterpret_cast<float4*>(wo + (size_t)r * HD + d) = x;
-            if (d == 0) wml[r] = make_float2(M, L);
         }
-    }
-    if (ns == 1) return;
-    // ---- pieces of one request and head: the last to arrive adds them, in order
-    __threadfence();
-    __syncthreads();
-    int* ticket = reinterpret_cast<int*>(a.work + a.l.tick) + first;
-    if (threadIdx.x == 0) {
-        const int last = atomicAdd(ticket, 1) == ns - 1;
-        if (last) *ticket = 0;                                     // ready for the next layer
-        *s_last = last;
-    }
-    __syncthreads();
-    if (!*s_last) return;
-    __threadfence();
-    const float* po = reinterpret_cast<const float*>(a.work + a.l.dec_part) + (size_t)first * kDecRows * HD;
-    const float2* pml = reinterpret_cast<const float2*>(a.work + a.l.dec_ml) + (size_t)first * kDecRows;
-    const size_t so = (size_t)NKV * kDecRows * HD, sm = (size_t)NKV * kDecRows;
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
-        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        float M = -INFINITY, L = 0.0f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = 0; s0 < ns; s0 += 8) {                       // eight pieces' loads in flight
-            float2 ml[8];
-            float4 y[8];
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const int s = min(s0 + u, ns - 1);
-                ml[u] = __ldcg(pml + s * sm + r);
-                y[u] = __ldcg(reinterpret_cast<const float4*>(po + s * so + (size_t)r * HD + d));
-            }
-            float mn = M;
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                if (s0 + u >= ns) ml[u] = make_float2(-INFINITY, 0.0f);
-                mn = fmaxf(mn, ml[u].x);
-            }
-            if (mn == -INFINITY) continue;
-            const float g = M == -INFINITY ? 0.0f : fast_exp2(M - mn);
-            M = mn;
-            L *= g;
-            x.x *= g; x.y *= g; x.z *= g; x.w *= g;
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float f = ml[u].x == -INFINITY ? 0.0f : fast_exp2(ml[u].x - mn);
-                L = fmaf(f, ml[u].y, L);
-                x.x = fmaf(f, y[u].x, x.x); x.y = fmaf(f, y[u].y, x.y); x.z = fmaf(f, y[u].z, x.z); x.w = fmaf(f, y[u].w, x.w);
-            }
-        }
-        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-        store(r, d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
     }
 }
 
-template <int HD>
+template <int HD, int NT>
 cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
-    using C = DecCfg<HD>;
+    using C = DecCfg<HD, NT>;
     constexpr int smem = C::SMEM + 1024;
+    constexpr int resident = dec_ctas_per_sm(HD, NT == 2);
+    static_assert(resident * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
     static std::once_flag once[kMaxDevices];
     static cudaError_t status[kMaxDevices];
     const cudaError_t e = once_per_device(once, status, [] {
-        const cudaError_t x = cudaFuncSetAttribute(paged_decode_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        return x != cudaSuccess ? x : cudaFuncSetAttribute(paged_decode_kernel<HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return cudaFuncSetAttribute(paged_decode_kernel<HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
     if (e != cudaSuccess) return e;
     CUtensorMap tmk, tmv;
@@ -494,19 +570,19 @@ cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
     if (!encode_tmap_2d(&tmk, a.kv.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz) ||
         !encode_tmap_2d(&tmv, a.kv.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz))
         return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)(a.l.dec_cap * a.kv.n_kv_head));
-    if (a.l.few <= 8) return launch_pdl(paged_decode_kernel<HD, 1>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
-    return launch_pdl(paged_decode_kernel<HD, 2>, grid, dim3(kThreads), (size_t)smem, st, tmk, tmv, a);
+    return launch_pdl(paged_decode_kernel<HD, NT>, dim3((unsigned)(a.l.dec_slots * a.kv.n_kv_head)), dim3(kThreads), (size_t)smem, st,
+                      tmk, tmv, a);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_decode(const PagedAttn& a, cudaStream_t st) {
     if (a.l.dec_cap == 0) return cudaSuccess;
+    const bool two = a.l.few > 8;
     switch (a.kv.head_dim) {
-        case 64: return launch_hd<64>(a, st);
-        case 128: return launch_hd<128>(a, st);
-        default: return launch_hd<256>(a, st);
+        case 64: return two ? launch_hd<64, 2>(a, st) : launch_hd<64, 1>(a, st);
+        case 128: return two ? launch_hd<128, 2>(a, st) : launch_hd<128, 1>(a, st);
+        default: return two ? launch_hd<256, 2>(a, st) : launch_hd<256, 1>(a, st);
     }
 }
 

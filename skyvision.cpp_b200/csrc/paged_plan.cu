@@ -196,37 +196,58 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
     } else {
         // ---- per request
         int4* req = reinterpret_cast<int4*>(work + a.l.req);
-        for (int r = threadIdx.x; r < n; r += kThreads) {
+        auto req_of = [&](int r) {
             const int p = past[r], c = start[r + 1] - start[r], held = (p + ps - 1) >> lg;
             const int got = min(max(nf - taken[r], 0), taken[r + 1] - taken[r]);
-            const int len = (int)min((long long)p + c, ((long long)held + got) << lg);
-            s.q_start[r] = start[r];
-            s.kv_len[r] = len;
-            req[r] = make_int4(start[r], c, p, len);
+            return make_int4(start[r], c, p, (int)min((long long)p + c, ((long long)held + got) << lg));
+        };
+        for (int r = threadIdx.x; r < n; r += kThreads) {
+            const int4 q = req_of(r);
+            s.q_start[r] = q.x;
+            s.kv_len[r] = q.w;
+            req[r] = q;
         }
         if (threadIdx.x == 0) {
             s.q_start[n] = start[n];
             *a.n_free_out = max(nf - taken[n], 0);
         }
         for (int i = threadIdx.x; i < a.l.n_ticks; i += kThreads) reinterpret_cast<int*>(work + a.l.tick)[i] = 0;
-        // ---- decode items: requests of few rows, their keys in splits
-        int2* dec = reinterpret_cast<int2*>(work + a.l.dec);
+        // ---- decode: the key tiles of all requests of few rows form one line, cut into equal pieces, a CTA each; a
+        // piece's part of a request is a segment
+        int4* dec = reinterpret_cast<int4*>(work + a.l.dec);
+        int* cta = reinterpret_cast<int*>(work + a.l.cta);
         auto dec_cost = [&](int r) {
             const int c = start[r + 1] - start[r];
             if (c == 0 || c * a.G > a.l.few) return 0;
             return (past[r] + c + kDecTile - 1) / kDecTile;
         };
-        int base = 0;
-        {
-            const int piece = piece_of(n, a.l.dec_slots, kDecMinTiles, dec_cost, buf);
+        if (a.l.dec_cap > 0) {
+            long long line;
+            {
+                long long sum = 0;
+                for (int r = threadIdx.x; r < n; r += kThreads) sum += dec_cost(r);
+                block_scan<long long>(sum, &line, buf);
+            }
+            const long long even = (line + a.l.dec_slots - 1) / a.l.dec_slots;
+            const long long piece = even < kDecMinTiles ? kDecMinTiles : even;
+            long long t0 = 0;
+            int base = 0;
             for (int u0 = 0; u0 < n; u0 += kThreads) {
                 const int r = u0 + threadIdx.x;
-                const int c = r < n ? dec_cost(r) : 0;
-                const int ns = (c + piece - 1) / piece;
-                long long all, at = block_scan<long long>(ns, &all, buf);
-                for (int i = 0; i < ns; i++) dec[base + at + i] = make_int2(r, i | ns << 16);
+                const long long c = r < n ? dec_cost(r) : 0;
+                long long all, t = t0 + block_scan<long long>(c, &all, buf);
+                t0 += all;
+                const int ns = c > 0 ? (int)((t + c - 1) / piece - t / piece) + 1 : 0;
+                const int at = base + (int)block_scan<long long>(ns, &all, buf);
                 base += (int)all;
+                for (int i = 0; i < ns; i++) {
+                    const long long lo = (t / piece + i) * piece, g0 = lo > t ? lo : t, g1 = lo + piece < t + c ? lo + piece : t + c;
+                    dec[2 * (at + i)] = make_int4(r, (int)(g0 - t), (int)(g1 - t), i | ns << 16);
+                    dec[2 * (at + i) + 1] = req_of(r);
+                    if (g0 == lo) cta[lo / piece] = at + i;
+                }
             }
+            for (long long i = (line + piece - 1) / piece + threadIdx.x; i <= a.l.dec_slots; i += kThreads) cta[i] = base;
         }
         // ---- prefill items: query tiles of the other requests, last ones (most keys) first
         int4* pre = reinterpret_cast<int4*>(work + a.l.pre);
@@ -254,7 +275,6 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
         if (threadIdx.x == 0) {
             int* head = reinterpret_cast<int*>(work + a.l.head);
             head[PH_PAGES] = touched[n];
-            head[PH_DEC] = base;
             head[PH_PRE] = pbase;
         }
     }
@@ -311,11 +331,11 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     const int64_t T = s.n_tokens, act = s.n_req < T ? s.n_req : T;
     const int max_new = s.max_new < T ? s.max_new : (int)T;
     l->page_cap = (int)(T < T / ps + 2 * act ? T : T / ps + 2 * act);
-    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    l->dec_slots = (int)up((int64_t)sms * dec_ctas_per_sm(s.head_dim), s.n_kv_head);
     l->few = few_rows((int64_t)max_new * G);
+    const int dec_ctas = sms * dec_ctas_per_sm(s.head_dim, l->few > 8);       // no more than run at once
+    l->dec_slots = dec_ctas > s.n_kv_head ? dec_ctas / s.n_kv_head : 1;
     l->dec_cap = G <= l->few ? (int)(act + l->dec_slots) : 0;
-    l->pre_slots = (int)up(sms, s.n_kv_head);
+    l->pre_slots = sms > s.n_kv_head ? sms / s.n_kv_head : 1;
     const int rows = pre_rows(s.head_dim);
     if ((int64_t)max_new * G > l->few) {
         const int64_t least = l->few / G + 1;    // fewest tokens of a prefill request
@@ -331,7 +351,8 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     l->head = take(128);
     l->req = take(sizeof(int4) * (size_t)s.n_req);
     l->page = take(sizeof(int4) * (size_t)l->page_cap);
-    l->dec = take(sizeof(int2) * (size_t)l->dec_cap);
+    l->dec = take(2 * sizeof(int4) * (size_t)l->dec_cap);
+    l->cta = take(sizeof(int) * (size_t)(l->dec_slots + 1));
     l->pre = take(sizeof(int4) * (size_t)l->pre_cap);
     l->tick = take(sizeof(int) * (size_t)l->n_ticks);
     l->dec_part = take(sizeof(float) * (size_t)l->dec_cap * s.n_kv_head * kDecRows * s.head_dim);
