@@ -9,12 +9,16 @@
 //
 // Work item (from the plan): NQT tiles of 128 rows of one request and kv head (rows = tokens x the G query
 // heads, packed, so any G fills them) x a piece of the keys they see.  Roles:
-//   softmax warps   4 per row tile, one row per thread: S from TMEM, scales, causal / window mask, maximum, P as
-//                   f16 back over the S columns.  m_r is lazy: it moves (and O is rescaled in TMEM) only when
-//                   a row of the warp passes it by 2^8, so most tiles never touch O.
-//   converter warps read code tiles (16 bytes a thread, straight from the pages), turn bytes into f16 by
-//                   permutes (0x64uu = 1024 + u; minus 1152 is exact) and write them 128-byte swizzled into
-//                   a ring of K and V tiles; the loads of the next tile are issued as each piece is stored.
+//   softmax warps   4 per row tile, one row per thread: S from TMEM, scales, causal / window mask, P as f16 back
+//                   over the S columns, 64 keys at a time so that O += P V starts on the first half.  No maximum
+//                   is taken as a rule: the weights are formed against the m_r at hand, and only where a row's sum
+//                   over the 64 keys passes 2^10 (far inside f16) or a row has no m_r yet is the maximum found, O in
+//                   TMEM and the sum rescaled, and the half formed again.
+//                   The V scales ride in the exponent: p' = exp2(x + log2 vs - v_ref), and the row sum takes each
+//                   group's share times 2^(v_ref - log2 vs), so they cost nothing per weight.
+//   converter warps read code tiles straight from the pages, turn bytes into f16 by permutes (0x64uu = 1024 + u;
+//                   minus 1152 is exact) and write them 128-byte swizzled into a ring of K and V tiles; the
+//                   loads of the next tile are issued as each piece is stored.
 //   MMA thread      S = Q K^T (both K-major), O += P V (P from TMEM, V MN-major).
 // With two row tiles (HD 64, 128; 128 keys) each has one S buffer and they alternate on the tensor core; with
 // one (HD 256; 64 keys) S is double-buffered.
@@ -29,7 +33,9 @@ namespace svkv {
 
 namespace {
 
-constexpr float kLazyLog2 = 8.0f;
+constexpr float kSumLimit = 1024.0f;      // a row's sum over 64 keys against its m_r; p' stays below 4 of it
+constexpr float kVRefSlack = 2.0f;        // log2 vs may pass v_ref by this much before O is rescaled
+constexpr float kVFloor = -40.0f;         // log2 of the smallest vs / v_ref told apart (pages of zeros have vs = 0)
 
 template <int HD>
 struct PreCfgP {
@@ -51,9 +57,10 @@ struct PreCfgP {
     static constexpr int THREADS = SPLIT_REGS ? 512 : (SM_WARPS + CV_WARPS + 1) * 32;
     static constexpr int GROUPS = BN / 16;                // 16-key groups of a tile
     static constexpr int OFF_RING = NQT * Q_B;
-    static constexpr int OFF_SC = OFF_RING + NE * KV_B;   // float2 [SM_WARPS][2][32]
-    static constexpr int OFF_BAR = OFF_SC + SM_WARPS * 2 * 32 * 8;
-    static constexpr int N_BAR = 2 * NE + 1 + NQT * 6;
+    static constexpr int HALVES = BN / 64;
+    static constexpr int OFF_SC = OFF_RING + NE * KV_B;   // float4 [SM_WARPS][32]
+    static constexpr int OFF_BAR = OFF_SC + SM_WARPS * 32 * 16;
+    static constexpr int N_BAR = 2 * NE + 1 + NQT * 9;
     static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 32;
     static_assert(SMEM + 1024 <= 227 * 1024, "shared memory budget");
     static constexpr int SCOLS = 128;                     // S/P columns per row tile, O after them
@@ -95,8 +102,9 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
     uint64_t* empty = bars + C::NE;             // [NE] MMA -> converters
     uint64_t* q_full = bars + 2 * C::NE;
     uint64_t* s_full = q_full + 1;              // [NQT][2]
-    uint64_t* p_full = s_full + 2 * C::NQT;     // [NQT][2]
-    uint64_t* o_done = p_full + 2 * C::NQT;     // [NQT][2]
+    uint64_t* p_full = s_full + 2 * C::NQT;     // [NQT][2][2]: P of a 64-key half, by the tile's parity
+    uint64_t* o_done = p_full + 4 * C::NQT;     // [NQT][2]
+    uint64_t* o_half = o_done + 2 * C::NQT;     // [NQT]: O has the tile's first half
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::N_BAR);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* s_last = abort_flag + 1;
@@ -129,9 +137,11 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
         mbar_init(q_full, 4 * C::NQT);
         for (int i = 0; i < 2 * C::NQT; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
             mbar_init(&o_done[i], 1);
         }
+        for (int i = 0; i < C::NQT; i++) mbar_init(&o_half[i], 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -184,9 +194,9 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        // Scales of 32 groups at a time in this warp's own table: x = ks scale log2(e) (a page of zeros has
-        // zero scores at any x > 0), y = vs; a group without a page has x < 0.
-        float2* sc = reinterpret_cast<float2*>(smem + C::OFF_SC) + warp * 64;
+        // Scales of 32 groups at a time in this warp's own table: x = ks scale log2(e) (a page of zeros has zero
+        // scores at any x > 0; a group without a page has x < 0), y = log2 vs - v_ref, z = 2^-y.
+        float4* tab = reinterpret_cast<float4*>(smem + C::OFF_SC) + warp * 32;
         constexpr int TPB = 32 / C::GROUPS;                 // tiles per batch of 32 groups
         auto scale_of = [&](int g, int p) {
             float2 s = make_float2(-1.0f, 0.0f);
@@ -199,19 +209,30 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
         int pg = page_of(j0 * C::GROUPS + lane);
         float2 next = scale_of(j0 * C::GROUPS + lane, pg);
         pg = page_of(j0 * C::GROUPS + 32 + lane);
-        float m = -INFINITY, vref = 0.0f;
-        float2 l2 = make_float2(0.0f, 0.0f);
+        float m = -INFINITY, l = 0.0f, vref = -INFINITY;
+        unsigned holes = 0;                                 // groups of the batch without a page
         bool ok = true;
         const int n_mine = tile_live ? n : 0;
-        for (int i = 0; i < n_mine; i++) {
+        for (int i = 0; i < n_mine && ok; i++) {
             const int at = (i % TPB) * C::GROUPS;
-            float2* tab = sc + ((i / TPB) & 1) * 32;
+            float vmove = 1.0f;                             // factor on O when v_ref moves
             if (at == 0) {
-                tab[lane] = next;
-                const int g = (j0 + i) * C::GROUPS + 32 + lane;
-                if (next.x < 0.0f && g - 32 < g_stop && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
-                next = scale_of(g, pg);
-                pg = page_of(g + 32);
+                const int g = (j0 + i) * C::GROUPS + lane;
+                const float lv = next.y > 0.0f ? __log2f(next.y) : -INFINITY;
+                float vm = lv;
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, w));
+                if (vm > vref + kVRefSlack) {
+                    if (vref > -INFINITY) vmove = fast_exp2(vref - vm);   // (zeros so far: O is 0)
+                    vref = vm;
+                }
+                const float y = fmaxf(lv - (vref > -INFINITY ? vref : 0.0f), kVFloor);
+                __syncwarp();
+                tab[lane] = make_float4(next.x, y, fast_exp2(-y), 0.0f);
+                holes = __ballot_sync(0xffffffffu, next.x < 0.0f);
+                if (next.x < 0.0f && g < g_stop && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
+                next = scale_of(g + 32, pg);
+                pg = page_of(g + 64);
                 __syncwarp();
             }
             const int sb = C::S2 ? i & 1 : 0;
@@ -219,87 +240,93 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
             tc_fence_after();
             const int kb = (j0 + i) * C::BN;
             const uint32_t sbuf = lane_addr + sb * C::BN;
-            float s[C::BN];
+            const bool edge = __any_sync(0xffffffffu, kb < lo || kb + C::BN > hi) || ((holes >> at) & ((1u << C::GROUPS) - 1)) != 0;
+            float s[C::HALVES][64];
 #pragma unroll
-            for (int cc = 0; cc < C::BN; cc += 32) tmem_ld32(sbuf + cc, s + cc);
-            float c[C::GROUPS], vmax = 0.0f;
-            bool hole = false;
-#pragma unroll
-            for (int g = 0; g < C::GROUPS; g++) {
-                c[g] = tab[at + g].x;
-                vmax = fmaxf(vmax, tab[at + g].y);
-                hole |= c[g] < 0.0f;
+            for (int hf = 0; hf < C::HALVES; hf++) {
+                tmem_ld32(sbuf + 64 * hf, s[hf]);
+                tmem_ld32(sbuf + 64 * hf + 32, s[hf] + 32);
             }
             tmem_wait_ld();
-            if (__any_sync(0xffffffffu, hole || kb < lo || kb + C::BN > hi)) {
 #pragma unroll
-                for (int k = 0; k < C::BN; k++)
-                    if (kb + k < lo || kb + k >= hi || c[k / 16] < 0.0f) s[k] = -INFINITY;
-#pragma unroll
-                for (int g = 0; g < C::GROUPS; g++) c[g] = fabsf(c[g]);
-            }
-            float mt = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < C::GROUPS; g++) {
-                float x = s[16 * g];
-#pragma unroll
-                for (int k = 1; k < 16; k++) x = fmaxf(x, s[16 * g + k]);
-                mt = fmaxf(mt, x * c[g]);
-            }
-            if (__any_sync(0xffffffffu, mt > m + kLazyLog2) || vmax > 4.0f * vref) {
-                const float mn = fmaxf(m, mt);
-                float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
-                m = mn;
-                l2 = make_float2(l2.x * f, l2.y * f);
-                if (vmax > vref) {
-                    f *= vref / vmax;
-                    vref = vmax;
-                }
-                if (i > 0) {
-                    if (!warp_wait(&o_done[2 * qtl + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int cc = 0; cc < HD; cc += 32) {
-                        float o[32];
-                        tmem_ld32(lane_addr + C::SCOLS + cc, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 32; k++) o[k] *= f;
-                        tmem_st32(lane_addr + C::SCOLS + cc, o);
-                    }
-                }
-            }
-            const float mneg = m == -INFINITY ? 0.0f : -m;
-            const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f;
-            const float2 mm = make_float2(mneg, mneg);
-#pragma unroll
-            for (int cc = 0; cc < C::BN; cc += 64) {
+            for (int hf = 0; hf < C::HALVES; hf++) {
                 uint32_t pk[32];
+                float sum = 0.0f;
+                auto mask = [&]() {                         // one row's visible keys of this half
+                    const int a0 = lo - kb - 64 * hf, a1 = hi - kb - 64 * hf;
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const float cg = c[cc / 16 + g], w = tab[at + cc / 16 + g].y * vinv;
-                    const float2 c2 = make_float2(cg, cg), w2 = make_float2(w, w);
+                    for (int k = 0; k < 64; k++)
+                        if (k < a0 || k >= a1 || ((holes >> (at + 4 * hf + k / 16)) & 1)) s[hf][k] = -INFINITY;
+                };
+                auto weights = [&]() {
+                    const float mneg = m == -INFINITY ? 0.0f : -m;
+                    sum = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 16; k += 2) {
-                        const float2 x = fma2(make_float2(s[cc + 16 * g + k], s[cc + 16 * g + k + 1]), c2, mm);
-                        const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-                        l2 = add2(l2, p);
-                        const float2 y = mul2(p, w2);
-                        pk[8 * g + k / 2] = pack_h2(y.x, y.y);
+                    for (int g = 0; g < 4; g++) {
+                        const float4 t = tab[at + 4 * hf + g];
+                        const float cg = fabsf(t.x), k0 = t.y + mneg;
+                        const float2 c2 = make_float2(cg, cg), kk = make_float2(k0, k0);
+                        float2 s2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int k = 0; k < 16; k += 2) {
+                            const float2 x = fma2(make_float2(s[hf][16 * g + k], s[hf][16 * g + k + 1]), c2, kk);
+                            const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                            s2 = add2(s2, p);
+                            pk[8 * g + k / 2] = pack_h2(p.x, p.y);
+                        }
+                        sum = fmaf(s2.x + s2.y, t.z, sum);
                     }
+                };
+                if (edge) mask();
+                weights();
+                if (__any_sync(0xffffffffu, !(sum <= kSumLimit) || m == -INFINITY) || (hf == 0 && vmove != 1.0f)) {
+                    // the rows' maxima over this half, O and the sums to match, and the half once more
+                    tmem_ld32(sbuf + 64 * hf, s[hf]);
+                    tmem_ld32(sbuf + 64 * hf + 32, s[hf] + 32);
+                    tmem_wait_ld();
+                    if (edge) mask();
+                    float mn = m;
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        float x = s[hf][16 * g];
+#pragma unroll
+                        for (int k = 1; k < 16; k++) x = fmaxf(x, s[hf][16 * g + k]);
+                        mn = fmaxf(mn, x * fabsf(tab[at + 4 * hf + g].x));
+                    }
+                    float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+                    m = mn;
+                    l *= f;
+                    if (hf == 0) f *= vmove;
+                    if (i > 0 || hf > 0) {                  // O must not be changing: the products issued so far are done
+                        const bool done = hf > 0 ? warp_wait(&o_half[qtl], i & 1, a.err, abort_flag)
+                                                 : warp_wait(&o_done[2 * qtl + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err, abort_flag);
+                        if (!done) { ok = false; break; }
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int cc = 0; cc < HD; cc += 32) {
+                            float o[32];
+                            tmem_ld32(lane_addr + C::SCOLS + cc, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k++) o[k] *= f;
+                            tmem_st32(lane_addr + C::SCOLS + cc, o);
+                        }
+                    }
+                    weights();
                 }
-                tmem_st32(sbuf + cc / 2, reinterpret_cast<const float*>(pk));
+                l += sum;
+                tmem_st32(sbuf + 32 * hf, reinterpret_cast<const float*>(pk));
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[4 * qtl + 2 * (i & 1) + hf]);
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * qtl + (i & 1)]);
         }
         if (n_mine > 0 && ok && !warp_wait(&o_done[2 * qtl + ((n_mine - 1) & 1)], ((n_mine - 1) >> 1) & 1, a.err, abort_flag))
             ok = false;
         tc_fence_after();
         const bool have = n_mine > 0 && ok;
-        const float l = l2.x + l2.y;
+        const float vscale = vref > -INFINITY ? fast_exp2(vref) : 1.0f;     // O is in units of it
         auto load_o = [&](int cc, float* o, float f) {
             if (have) {
                 tmem_ld32(lane_addr + C::SCOLS + cc, o);
@@ -328,7 +355,7 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
 #pragma unroll 1
             for (int cc = 0; cc < HD; cc += 32) {
                 float o[32];
-                load_o(cc, o, vref);
+                load_o(cc, o, vscale);
                 store(cc, o, inv);
             }
         } else {
@@ -340,7 +367,7 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
 #pragma unroll 1
             for (int cc = 0; cc < HD; cc += 32) {
                 float o[32];
-                load_o(cc, o, vref);
+                load_o(cc, o, vscale);
                 if (tile_live) {
 #pragma unroll
                     for (int k = 0; k < 8; k++)
@@ -394,53 +421,54 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
     } else if (warp < C::SM_WARPS + C::CV_WARPS) {
         // ============================ converters: entry e is K (even) or V (odd) of tile e / 2
         if constexpr (C::SPLIT_REGS) regs_down<80>();
+        // Eight threads per row, one 16-key group per pass: a thread turns the same 8 codes of every 64-column slab
+        // into one 16-byte column, so the eight columns of a row are written by one conflict-free store, and
+        // all its addresses are a group's base plus constants.
         const int t = threadIdx.x - C::SM_WARPS * 32;
-        constexpr int TPR = HD / 16;                        // threads per row, 16 codes each
-        constexpr int RPP = C::CV_WARPS * 32 / TPR;         // rows per pass
-        constexpr int PASSES = C::BN / RPP;
-        const int c16 = t % TPR, r0 = t / TPR;
-        // pages of 32 groups from the batch's first, and of the next 32 (a batch is whole tiles)
+        constexpr int SLABS = HD / 64;
+        const int j = t & 7, r = t >> 3;                    // piece of a slab's row, row of the group
+        const uint8_t* ksrc = static_cast<const uint8_t*>(a.kv.k) + (size_t)r * HD + 8 * j;
+        const uint8_t* vsrc = static_cast<const uint8_t*>(a.kv.v) + (size_t)r * HD + 8 * j;
+        const uint32_t to = r * 128 + ((j ^ (r & 7)) << 4);
+        // lane l: where group b0 + l lies in the pool, in groups (-1: nowhere), and its page in the next batch
+        auto place = [&](int g, int page) {
+            return g < g_stop && valid(page) ? ((page * NKV + h) << (lg - 4)) + (g & ((a.kv.page_size >> 4) - 1)) : -1;
+        };
         int b0 = j0 * C::GROUPS;
-        int p0 = page_of(b0 + lane), p1 = page_of(b0 + 32 + lane);
-        uint4 raw[PASSES];
-        auto fetch = [&](int e, int p) {
-            const int row = p * RPP + r0, key = (j0 + (e >> 1)) * C::BN + row;
-            const int page = __shfl_sync(0xffffffffu, p0, ((key >> 4) - b0) & 31);
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (e < 2 * n && (key >> 4) < g_stop && valid(page)) {
-                const uint8_t* src = static_cast<const uint8_t*>((e & 1) ? a.kv.v : a.kv.k);
-                x = __ldg(reinterpret_cast<const uint4*>(
-                    src + ((((size_t)page * NKV + h) << lg) + (key & (a.kv.page_size - 1))) * HD + c16 * 16));
-            }
-            return x;
+        int here = place(b0 + lane, page_of(b0 + lane)), p1 = page_of(b0 + 32 + lane);
+        uint2 raw[C::GROUPS][SLABS];
+        auto fetch = [&](int e, int g0, int p) {            // group p of entry e, whose tile starts at lane g0
+            const int g = __shfl_sync(0xffffffffu, here, g0 + p);
+            const uint8_t* src = ((e & 1) ? vsrc : ksrc) + (size_t)(unsigned)g * (16 * HD);
+#pragma unroll
+            for (int i = 0; i < SLABS; i++) raw[p][i] = g >= 0 ? __ldg(reinterpret_cast<const uint2*>(src + 64 * i)) : make_uint2(0, 0);
         };
         if (n > 0) {
 #pragma unroll
-            for (int p = 0; p < PASSES; p++) raw[p] = fetch(0, p);
+            for (int p = 0; p < C::GROUPS; p++) fetch(0, 0, p);
         }
         for (int e = 0; e < 2 * n; e++) {
             const int sl = e % C::NE;
             if (e >= C::NE && !warp_wait(&empty[sl], ((e / C::NE) - 1) & 1, a.err, abort_flag)) break;
-            // the next entry's tile may start in the next batch of groups
-            if ((j0 + ((e + 1) >> 1)) * C::GROUPS - b0 >= 32) {
+            // the next entry's tile may start the next batch of groups (a batch is whole tiles)
+            int g0 = (j0 + ((e + 1) >> 1)) * C::GROUPS - b0;
+            if (g0 >= 32) {
                 b0 += 32;
-                p0 = p1;
+                g0 -= 32;
+                here = place(b0 + lane, p1);
                 p1 = page_of(b0 + 32 + lane);
             }
-            uint8_t* dst = smem + C::OFF_RING + sl * C::KV_B + (c16 >> 2) * C::KBOX;
-            const int ch = (c16 & 3) * 2, swap = (c16 >> 2) & 1;
+            uint8_t* dst = smem + C::OFF_RING + sl * C::KV_B + to;
+            const bool more = e + 1 < 2 * n;
 #pragma unroll
-            for (int p = 0; p < PASSES; p++) {
-                const int row = p * RPP + r0;
-                const uint32_t w[4] = {raw[p].x ^ 0x80808080u, raw[p].y ^ 0x80808080u, raw[p].z ^ 0x80808080u, raw[p].w ^ 0x80808080u};
-                raw[p] = fetch(e + 1, p);
-                uint4 y[2];
-                y[0] = make_uint4(code_pair(w[0], 0x4140), code_pair(w[0], 0x4342), code_pair(w[1], 0x4140), code_pair(w[1], 0x4342));
-                y[1] = make_uint4(code_pair(w[2], 0x4140), code_pair(w[2], 0x4342), code_pair(w[3], 0x4140), code_pair(w[3], 0x4342));
-                // the eight threads of a store cover eight different 16-byte columns: half of them start with the second
-                uint8_t* base = dst + row * 128;
-                *reinterpret_cast<uint4*>(base + (((ch + swap) ^ (row & 7)) << 4)) = swap ? y[1] : y[0];
-                *reinterpret_cast<uint4*>(base + (((ch + 1 - swap) ^ (row & 7)) << 4)) = swap ? y[0] : y[1];
+            for (int p = 0; p < C::GROUPS; p++) {
+#pragma unroll
+                for (int i = 0; i < SLABS; i++) {
+                    const uint32_t x = raw[p][i].x ^ 0x80808080u, y = raw[p][i].y ^ 0x80808080u;
+                    *reinterpret_cast<uint4*>(dst + i * C::KBOX + p * 16 * 128) =
+                        make_uint4(code_pair(x, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4140), code_pair(y, 0x4342));
+                }
+                if (more) fetch(e + 1, g0, p);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -472,13 +500,17 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
             umma_commit(&s_full[2 * q + (i & 1)]);
         };
         auto mma_pv = [&](int i, int q) -> bool {
-            if (!wait_or_abort(&p_full[2 * q + (i & 1)], (i >> 1) & 1, a.err, abort_flag)) return false;
-            tc_fence_after();
             const uint32_t vd = v_lo + (uint32_t)(((2 * i + 1) % C::NE) * (C::KV_B >> 4));
             const uint32_t p = tmem + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0), o = tmem + q * C::QCOLS + C::SCOLS;
 #pragma unroll
-            for (int kk = 0; kk < C::BN / 16; kk++)
-                umma_f16_ts(o, p + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), hi, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+            for (int hf = 0; hf < C::HALVES; hf++) {
+                if (!wait_or_abort(&p_full[4 * q + 2 * (i & 1) + hf], (i >> 1) & 1, a.err, abort_flag)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
+                    umma_f16_ts(o, p + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), hi, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                if (hf + 1 < C::HALVES) umma_commit(&o_half[q]);
+            }
             umma_commit(&o_done[2 * q + (i & 1)]);
             return true;
         };
