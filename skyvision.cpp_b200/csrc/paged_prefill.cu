@@ -19,7 +19,7 @@
 //   converter warps read code tiles straight from the pages, turn bytes into f16 by permutes (0x64uu = 1024 + u;
 //                   minus 1152 is exact) and write them 128-byte swizzled into a ring of K and V tiles; the
 //                   loads of the next tile are issued as each piece is stored.
-//   MMA thread      S = Q K^T (both K-major), O += P V (P from TMEM, V MN-major).
+//   MMA warp        S = Q K^T (both K-major), O += P V (P from TMEM, V MN-major).
 // With two row tiles (HD 64, 128; 128 keys) each has one S buffer and they alternate on the tensor core; with
 // one (HD 256; 64 keys) S is double-buffered.
 // Pieces of an item's rows meet in the work space; the last to arrive adds them in order.
@@ -85,6 +85,13 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t sel) {
     const uint32_t h = __byte_perm(w, 0x64646464u, sel);
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
 }
 
 template <int N>
@@ -476,68 +483,81 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
         }
     } else {
         if constexpr (C::SPLIT_REGS) regs_down<48>();
-        if (warp == C::SM_WARPS + C::CV_WARPS && lane == 0 && n > 0) {
-        // ============================ MMA issuer
-        const uint32_t idesc_s = umma_idesc(128, C::BN, 0, 0), idesc_o = umma_idesc(128, HD, 0, 1);
-        constexpr uint32_t hi = desc_hi_sw128(1024);
-        const uint32_t q_lo = desc_lo(smem_u32(smem), 16);
-        const uint32_t k_lo = desc_lo(smem_u32(smem + C::OFF_RING), 16);
-        const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_RING), C::KBOX);
-        auto wait_full = [&](int e) {
-            const bool r = wait_or_abort(&full[e % C::NE], (e / C::NE) & 1, a.err, abort_flag);
-            tc_fence_after();
-            return r;
-        };
-        auto mma_s = [&](int i, int q) {
-            const uint32_t kd = k_lo + (uint32_t)(((2 * i) % C::NE) * (C::KV_B >> 4));
-            const uint32_t d = tmem + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0);
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; kk++) {
-                const uint32_t a_off = (uint32_t)((q * C::Q_B + (kk / 4) * C::QBOX + (kk % 4) * 32) >> 4);
-                const uint32_t b_off = (uint32_t)(((kk / 4) * C::KBOX + (kk % 4) * 32) >> 4);
-                umma_f16_w(d, q_lo + a_off, kd + b_off, hi, idesc_s, kk > 0 ? 1u : 0u);
-            }
-            umma_commit(&s_full[2 * q + (i & 1)]);
-        };
-        auto mma_pv = [&](int i, int q) -> bool {
-            const uint32_t vd = v_lo + (uint32_t)(((2 * i + 1) % C::NE) * (C::KV_B >> 4));
-            const uint32_t p = tmem + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0), o = tmem + q * C::QCOLS + C::SCOLS;
-#pragma unroll
-            for (int hf = 0; hf < C::HALVES; hf++) {
-                if (!wait_or_abort(&p_full[4 * q + 2 * (i & 1) + hf], (i >> 1) & 1, a.err, abort_flag)) return false;
+        const int nu = __shfl_sync(0xffffffffu, n, 0), nq = __shfl_sync(0xffffffffu, nqt, 0);
+        if (warp == C::SM_WARPS + C::CV_WARPS && nu > 0) {
+            // ======================== MMA issuer: the whole warp runs the loop and one elected lane issues, so that the
+            // descriptors are uniform values (held per thread they had to be moved to uniform registers before each MMA:
+            // 109 cycles between MMAs of 64)
+            const uint32_t idesc_s = umma_idesc(128, C::BN, 0, 0), idesc_o = umma_idesc(128, HD, 0, 1);
+            constexpr uint32_t hi = desc_hi_sw128(1024);
+            const uint32_t q_lo = desc_lo(smem_u32(smem), 16);
+            const uint32_t k_lo = desc_lo(smem_u32(smem + C::OFF_RING), 16);
+            const uint32_t v_lo = desc_lo(smem_u32(smem + C::OFF_RING), C::KBOX);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const bool lead = elect_one();
+            auto wait_full = [&](int e) {
+                const bool r = warp_wait(&full[e % C::NE], (e / C::NE) & 1, a.err, abort_flag);
                 tc_fence_after();
+                return r;
+            };
+            auto commit = [&](uint64_t* bar) {
+                if (lead) umma_commit(bar);
+            };
+            auto mma_s = [&](int i, int q) {
+                const uint32_t kd = k_lo + (uint32_t)(((2 * i) % C::NE) * (C::KV_B >> 4));
+                const uint32_t d = tm + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0);
+                if (lead) {
 #pragma unroll
-                for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
-                    umma_f16_ts(o, p + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), hi, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
-                if (hf + 1 < C::HALVES) umma_commit(&o_half[q]);
-            }
-            umma_commit(&o_done[2 * q + (i & 1)]);
-            return true;
-        };
-        bool ok = wait_or_abort(q_full, 0, a.err, abort_flag) && wait_full(0);
-        if (ok) {
-            for (int q = 0; q < nqt; q++) mma_s(0, q);
-            umma_commit(&empty[0]);
-        }
-        for (int i = 0; ok && i < n; i++) {
-            if (C::S2 && i + 1 < n) {                       // S(i+1) overlaps the softmax of tile i
-                ok = wait_full(2 * i + 2);
-                if (!ok) break;
-                mma_s(i + 1, 0);
-                umma_commit(&empty[(2 * i + 2) % C::NE]);
-            }
-            ok = wait_full(2 * i + 1);
-            for (int q = 0; q < nqt && ok; q++) {
-                ok = mma_pv(i, q);
-                if (!C::S2 && ok && i + 1 < n) {            // S_q(i+1) overwrites P_q(i), after P.V_q(i) on the same pipe
-                    if (q == 0) ok = wait_full(2 * i + 2);
-                    if (ok) mma_s(i + 1, q);
+                    for (int kk = 0; kk < HD / 16; kk++) {
+                        const uint32_t a_off = (uint32_t)((q * C::Q_B + (kk / 4) * C::QBOX + (kk % 4) * 32) >> 4);
+                        const uint32_t b_off = (uint32_t)(((kk / 4) * C::KBOX + (kk % 4) * 32) >> 4);
+                        umma_f16_w(d, q_lo + a_off, kd + b_off, hi, idesc_s, kk > 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[2 * q + (i & 1)]);
                 }
+                __syncwarp();
+            };
+            auto mma_pv = [&](int i, int q) -> bool {
+                const uint32_t vd = v_lo + (uint32_t)(((2 * i + 1) % C::NE) * (C::KV_B >> 4));
+                const uint32_t p = tm + q * C::QCOLS + (C::S2 ? (i & 1) * C::BN : 0), o = tm + q * C::QCOLS + C::SCOLS;
+#pragma unroll
+                for (int hf = 0; hf < C::HALVES; hf++) {
+                    if (!warp_wait(&p_full[4 * q + 2 * (i & 1) + hf], (i >> 1) & 1, a.err, abort_flag)) return false;
+                    tc_fence_after();
+                    if (lead) {
+#pragma unroll
+                        for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
+                            umma_f16_ts(o, p + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), hi, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                        umma_commit(hf + 1 < C::HALVES ? &o_half[q] : &o_done[2 * q + (i & 1)]);
+                    }
+                    __syncwarp();
+                }
+                return true;
+            };
+            bool ok = warp_wait(q_full, 0, a.err, abort_flag) && wait_full(0);
+            if (ok) {
+                for (int q = 0; q < nq; q++) mma_s(0, q);
+                commit(&empty[0]);
             }
-            if (!ok) break;
-            umma_commit(&empty[(2 * i + 1) % C::NE]);
-            if (!C::S2 && i + 1 < n) umma_commit(&empty[(2 * i + 2) % C::NE]);
-        }
+            for (int i = 0; ok && i < nu; i++) {
+                if (C::S2 && i + 1 < nu) {                  // S(i+1) overlaps the softmax of tile i
+                    ok = wait_full(2 * i + 2);
+                    if (!ok) break;
+                    mma_s(i + 1, 0);
+                    commit(&empty[(2 * i + 2) % C::NE]);
+                }
+                ok = wait_full(2 * i + 1);
+                for (int q = 0; q < nq && ok; q++) {
+                    ok = mma_pv(i, q);
+                    if (!C::S2 && ok && i + 1 < nu) {       // S_q(i+1) overwrites P_q(i), after P.V_q(i) on the same pipe
+                        if (q == 0) ok = wait_full(2 * i + 2);
+                        if (ok) mma_s(i + 1, q);
+                    }
+                }
+                if (!ok) break;
+                commit(&empty[(2 * i + 1) % C::NE]);
+                if (!C::S2 && i + 1 < nu) commit(&empty[(2 * i + 2) % C::NE]);
+            }
         }
     }
 
