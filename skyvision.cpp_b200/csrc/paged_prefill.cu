@@ -248,85 +248,97 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
             const int kb = (j0 + i) * C::BN;
             const uint32_t sbuf = lane_addr + sb * C::BN;
             const bool edge = __any_sync(0xffffffffu, kb < lo || kb + C::BN > hi) || ((holes >> at) & ((1u << C::GROUPS) - 1)) != 0;
-            float s[C::HALVES][64];
+            // 32 columns at a time: the next are on their way from TMEM while these become weights
+            constexpr int CH = C::BN / 32;
+            float s[2][32];
+            uint32_t pk[32];
+            float sum = 0.0f;
+            auto mask = [&](float* x, int c) {              // this row's visible keys of 32
+                const int a0 = lo - kb - 32 * c, a1 = hi - kb - 32 * c;
+                const unsigned hole = holes >> (at + 2 * c);
 #pragma unroll
-            for (int hf = 0; hf < C::HALVES; hf++) {
-                tmem_ld32(sbuf + 64 * hf, s[hf]);
-                tmem_ld32(sbuf + 64 * hf + 32, s[hf] + 32);
-            }
+                for (int k = 0; k < 32; k++)
+                    if (k < a0 || k >= a1 || ((hole >> (k / 16)) & 1)) x[k] = -INFINITY;
+            };
+            auto weights = [&](const float* x, int c, uint32_t* w) {
+                const float mneg = m == -INFINITY ? 0.0f : -m;
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const float4 t = tab[at + 2 * c + g];
+                    const float cg = fabsf(t.x), k0 = t.y + mneg;
+                    const float2 c2 = make_float2(cg, cg), kk = make_float2(k0, k0);
+                    float2 s2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        const float2 y = fma2(make_float2(x[16 * g + k], x[16 * g + k + 1]), c2, kk);
+                        const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        s2 = add2(s2, p);
+                        w[8 * g + k / 2] = pack_h2(p.x, p.y);
+                    }
+                    sum = fmaf(s2.x + s2.y, t.z, sum);
+                }
+            };
+            tmem_ld32(sbuf, s[0]);
             tmem_wait_ld();
 #pragma unroll
-            for (int hf = 0; hf < C::HALVES; hf++) {
-                uint32_t pk[32];
-                float sum = 0.0f;
-                auto mask = [&]() {                         // one row's visible keys of this half
-                    const int a0 = lo - kb - 64 * hf, a1 = hi - kb - 64 * hf;
-#pragma unroll
-                    for (int k = 0; k < 64; k++)
-                        if (k < a0 || k >= a1 || ((holes >> (at + 4 * hf + k / 16)) & 1)) s[hf][k] = -INFINITY;
-                };
-                auto weights = [&]() {
-                    const float mneg = m == -INFINITY ? 0.0f : -m;
-                    sum = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        const float4 t = tab[at + 4 * hf + g];
-                        const float cg = fabsf(t.x), k0 = t.y + mneg;
-                        const float2 c2 = make_float2(cg, cg), kk = make_float2(k0, k0);
-                        float2 s2 = make_float2(0.0f, 0.0f);
-#pragma unroll
-                        for (int k = 0; k < 16; k += 2) {
-                            const float2 x = fma2(make_float2(s[hf][16 * g + k], s[hf][16 * g + k + 1]), c2, kk);
-                            const float2 p = make_float2(fast_exp2(x.x), fast_exp2(x.y));
-                            s2 = add2(s2, p);
-                            pk[8 * g + k / 2] = pack_h2(p.x, p.y);
-                        }
-                        sum = fmaf(s2.x + s2.y, t.z, sum);
-                    }
-                };
-                if (edge) mask();
-                weights();
-                if (__any_sync(0xffffffffu, !(sum <= kSumLimit) || m == -INFINITY) || (hf == 0 && vmove != 1.0f)) {
-                    // the rows' maxima over this half, O and the sums to match, and the half once more
-                    tmem_ld32(sbuf + 64 * hf, s[hf]);
-                    tmem_ld32(sbuf + 64 * hf + 32, s[hf] + 32);
-                    tmem_wait_ld();
-                    if (edge) mask();
-                    float mn = m;
-#pragma unroll
-                    for (int g = 0; g < 4; g++) {
-                        float x = s[hf][16 * g];
-#pragma unroll
-                        for (int k = 1; k < 16; k++) x = fmaxf(x, s[hf][16 * g + k]);
-                        mn = fmaxf(mn, x * fabsf(tab[at + 4 * hf + g].x));
-                    }
-                    float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
-                    m = mn;
-                    l *= f;
-                    if (hf == 0) f *= vmove;
-                    if (i > 0 || hf > 0) {                  // O must not be changing: the products issued so far are done
-                        const bool done = hf > 0 ? warp_wait(&o_half[qtl], i & 1, a.err, abort_flag)
-                                                 : warp_wait(&o_done[2 * qtl + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err, abort_flag);
-                        if (!done) { ok = false; break; }
-                        tc_fence_after();
+            for (int c = 0; c < CH; c++) {
+                const int hf = c / 2;
+                if (c + 1 < CH) tmem_ld32(sbuf + 32 * (c + 1), s[(c + 1) & 1]);
+                if (edge) mask(s[c & 1], c);
+                weights(s[c & 1], c, pk + 16 * (c & 1));
+                if (c & 1) {
+                    if (__any_sync(0xffffffffu, !(sum <= kSumLimit) || m == -INFINITY) || (hf == 0 && vmove != 1.0f)) {
+                        // the rows' maxima over this half, O and the sums to match, and the half once more
+                        float t[32], mn = m;
 #pragma unroll 1
-                        for (int cc = 0; cc < HD; cc += 32) {
-                            float o[32];
-                            tmem_ld32(lane_addr + C::SCOLS + cc, o);
+                        for (int k = 2 * hf; k < 2 * hf + 2; k++) {
+                            tmem_ld32(sbuf + 32 * k, t);
                             tmem_wait_ld();
+                            if (edge) mask(t, k);
 #pragma unroll
-                            for (int k = 0; k < 32; k++) o[k] *= f;
-                            tmem_st32(lane_addr + C::SCOLS + cc, o);
+                            for (int g = 0; g < 2; g++) {
+                                float x = t[16 * g];
+#pragma unroll
+                                for (int j = 1; j < 16; j++) x = fmaxf(x, t[16 * g + j]);
+                                mn = fmaxf(mn, x * fabsf(tab[at + 2 * k + g].x));
+                            }
+                        }
+                        float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+                        m = mn;
+                        l *= f;
+                        if (hf == 0) f *= vmove;
+                        if (i > 0 || hf > 0) {              // O must not be changing: the products issued so far are done
+                            const bool done = hf > 0 ? warp_wait(&o_half[qtl], i & 1, a.err, abort_flag)
+                                                     : warp_wait(&o_done[2 * qtl + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err, abort_flag);
+                            if (!done) { ok = false; break; }
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int cc = 0; cc < HD; cc += 32) {
+                                tmem_ld32(lane_addr + C::SCOLS + cc, t);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 32; k++) t[k] *= f;
+                                tmem_st32(lane_addr + C::SCOLS + cc, t);
+                            }
+                        }
+                        sum = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            tmem_ld32(sbuf + 64 * hf + 32 * k, t);
+                            tmem_wait_ld();
+                            if (edge) mask(t, 2 * hf + k);
+                            weights(t, 2 * hf + k, pk + 16 * k);
                         }
                     }
-                    weights();
+                    l += sum;
+                    sum = 0.0f;
+                    tmem_st32(sbuf + 32 * hf, reinterpret_cast<const float*>(pk));
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[4 * qtl + 2 * (i & 1) + hf]);
                 }
-                l += sum;
-                tmem_st32(sbuf + 32 * hf, reinterpret_cast<const float*>(pk));
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[4 * qtl + 2 * (i & 1) + hf]);
+                if (c + 1 < CH) tmem_wait_ld();
             }
         }
         if (n_mine > 0 && ok && !warp_wait(&o_done[2 * qtl + ((n_mine - 1) & 1)], ((n_mine - 1) >> 1) & 1, a.err, abort_flag))
