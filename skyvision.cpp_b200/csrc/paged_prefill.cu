@@ -18,7 +18,7 @@
 //                   group's share times 2^(v_ref - log2 vs), so they cost nothing per weight.
 //   converter warps read code tiles straight from the pages, turn bytes into f16 by permutes (0x64uu = 1024 + u;
 //                   minus 1152 is exact) and write them 128-byte swizzled into a ring of K and V tiles; the
-//                   loads of the next tile are issued as each piece is stored.
+//                   loads of the next tile are issued as each piece of this one is stored.
 //   MMA warp        S = Q K^T (both K-major), O += P V (P from TMEM, V MN-major).
 // With two row tiles (HD 64, 128; 128 keys) each has one S buffer and they alternate on the tensor core; with
 // one (HD 256; 64 keys) S is double-buffered.
@@ -33,6 +33,7 @@ namespace svkv {
 
 namespace {
 
+constexpr int kPolyOf4 = 0;               // exponentials of four that run on the FMA pipe
 constexpr float kSumLimit = 1024.0f;      // a row's sum over 64 keys against its m_r; p' stays below 4 of it
 constexpr float kVRefSlack = 2.0f;        // log2 vs may pass v_ref by this much before O is rescaled
 constexpr float kVFloor = -40.0f;         // log2 of the smallest vs / v_ref told apart (pages of zeros have vs = 0)
@@ -47,20 +48,23 @@ struct PreCfgP {
     static constexpr int Q_B = (HD / 64) * QBOX;
     static constexpr int KBOX = BN * 128;                 // one 64-column slab of a K or V tile
     static constexpr int KV_B = (HD / 64) * KBOX;
-    static constexpr int FIT = (227 * 1024 - 6144 - NQT * Q_B) / KV_B;
-    static constexpr int NE = FIT > 8 ? 8 : FIT;          // ring entries: K0 V0 K1 V1 ...
+    static constexpr int NE = HD == 64 ? 8 : HD == 128 ? 4 : 3;   // f16 ring entries: K0 V0 K1 V1 ...
+    static constexpr int RAW_B = 64 * HD;                 // codes of 64 keys: half an entry, or one
+    static constexpr int NR = HD == 64 ? 8 : 3;           // code ring entries, in the same order
+    static constexpr int COLS = HD < 128 ? HD : 128;      // bytes of one box row of codes
     static constexpr int SM_WARPS = 4 * NQT;
     static constexpr int CV_WARPS = 4;
     // Two row tiles: four warpgroups of 128 registers a thread at launch, split again by need
-    // (256 x 192 + 128 x 80 + 128 x 48 = 512 x 128).  One row tile fits as it is.
+    // (256 x 176 + 128 x 88 + 128 x 72 = 512 x 128).  One row tile fits as it is.
     static constexpr bool SPLIT_REGS = NQT == 2;
-    static constexpr int THREADS = SPLIT_REGS ? 512 : (SM_WARPS + CV_WARPS + 1) * 32;
+    static constexpr int THREADS = SPLIT_REGS ? 512 : (SM_WARPS + CV_WARPS + 2) * 32;
     static constexpr int GROUPS = BN / 16;                // 16-key groups of a tile
     static constexpr int OFF_RING = NQT * Q_B;
     static constexpr int HALVES = BN / 64;
-    static constexpr int OFF_SC = OFF_RING + NE * KV_B;   // float4 [SM_WARPS][32]
+    static constexpr int OFF_RAW = OFF_RING + NE * KV_B;
+    static constexpr int OFF_SC = OFF_RAW + NR * RAW_B;   // float4 [SM_WARPS][32]
     static constexpr int OFF_BAR = OFF_SC + SM_WARPS * 32 * 16;
-    static constexpr int N_BAR = 2 * NE + 1 + NQT * 9;
+    static constexpr int N_BAR = 2 * NE + 2 * NR + 1 + NQT * 9;
     static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 32;
     static_assert(SMEM + 1024 <= 227 * 1024, "shared memory budget");
     static constexpr int SCOLS = 128;                     // S/P columns per row tile, O after them
@@ -94,20 +98,39 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
+// 2^x of two values on the FMA pipe: x = n + f, f in [-1/2, 1/2], 2^f by the polynomial that the f16-cache prefill uses
+// (degree 4, fitted for minimax relative error, 2.7e-6), n added into the exponent.  Below -126 it gives 2^-126 or
+// less (0 in f16); x is below 126 (kSumLimit is checked on the exponentials of the other pipe as well).
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    x = make_float2(fminf(fmaxf(x.x, -126.0f), 126.0f), fminf(fmaxf(x.y, -126.0f), 126.0f));
+    const float2 magic = make_float2(12582912.0f, 12582912.0f), minus = make_float2(-12582912.0f, -12582912.0f);
+    const float2 t = add2(x, magic), f = add2(x, mul2(add2(t, minus), make_float2(-1.0f, -1.0f)));
+    float2 p = fma2(make_float2(0.00956530869f, 0.00956530869f), f, make_float2(0.05591748655f, 0.05591748655f));
+    p = fma2(p, f, make_float2(0.2402486354f, 0.2402486354f));
+    p = fma2(p, f, make_float2(0.6931219101f, 0.6931219101f));
+    p = fma2(p, f, make_float2(0.9999992251f, 0.9999992251f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int HD>
-__global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(const __grid_constant__ PagedAttn a) {
+__global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1)
+paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                     const __grid_constant__ PagedAttn a) {
     using C = PreCfgP<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* full = bars;                      // [NE] converters -> MMA
     uint64_t* empty = bars + C::NE;             // [NE] MMA -> converters
-    uint64_t* q_full = bars + 2 * C::NE;
+    uint64_t* raw_full = bars + 2 * C::NE;      // [NR] TMA -> converters
+    uint64_t* raw_empty = raw_full + C::NR;     // [NR] converters -> TMA
+    uint64_t* q_full = raw_empty + C::NR;
     uint64_t* s_full = q_full + 1;              // [NQT][2]
     uint64_t* p_full = s_full + 2 * C::NQT;     // [NQT][2][2]: P of a 64-key half, by the tile's parity
     uint64_t* o_done = p_full + 4 * C::NQT;     // [NQT][2]
@@ -141,6 +164,10 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
             mbar_init(&full[s], C::CV_WARPS);
             mbar_init(&empty[s], 1);
         }
+        for (int s = 0; s < C::NR; s++) {
+            mbar_init(&raw_full[s], 1);
+            mbar_init(&raw_empty[s], C::CV_WARPS);
+        }
         mbar_init(q_full, 4 * C::NQT);
         for (int i = 0; i < 2 * C::NQT; i++) {
             mbar_init(&s_full[i], 1);
@@ -170,7 +197,7 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
 
     if (warp < C::SM_WARPS) {
         // ============================ softmax: one row per thread
-        if constexpr (C::SPLIT_REGS) regs_up<192>();
+        if constexpr (C::SPLIT_REGS) regs_up<176>();
         const int qtl = warp >> 2, quarter = warp & 3;
         const bool tile_live = qtl < nqt;
         const int r = quarter * 32 + lane, flat = qtl * 128 + r;
@@ -271,7 +298,7 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
                         const float2 y = fma2(make_float2(x[16 * g + k], x[16 * g + k + 1]), c2, kk);
-                        const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        const float2 p = (k / 2) % 4 < kPolyOf4 ? exp2_poly(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
                         s2 = add2(s2, p);
                         w[8 * g + k / 2] = pack_h2(p.x, p.y);
                     }
@@ -333,10 +360,13 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
                     l += sum;
                     sum = 0.0f;
                     tmem_st32(sbuf + 32 * hf, reinterpret_cast<const float*>(pk));
+                }
+                // P is announced a chunk after it was stored (the last at once): the store is done by then
+                if ((c & 1) == 0 ? c > 0 : c + 1 == CH) {
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[4 * qtl + 2 * (i & 1) + hf]);
+                    if (lane == 0) mbar_arrive(&p_full[4 * qtl + 2 * (i & 1) + (c - 1) / 2]);
                 }
                 if (c + 1 < CH) tmem_wait_ld();
             }
@@ -439,64 +469,83 @@ __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1) paged_prefill_kernel(
         }
     } else if (warp < C::SM_WARPS + C::CV_WARPS) {
         // ============================ converters: entry e is K (even) or V (odd) of tile e / 2
-        if constexpr (C::SPLIT_REGS) regs_down<80>();
-        // Eight threads per row, one 16-key group per pass: a thread turns the same 8 codes of every 64-column slab
-        // into one 16-byte column, so the eight columns of a row are written by one conflict-free store, and
-        // all its addresses are a group's base plus constants.
+        if constexpr (C::SPLIT_REGS) regs_down<88>();
+        // A thread turns 8 codes into one 16-byte column of an f16 row: HD/8 threads per row, so that a half warp reads
+        // 128 bytes in a row and a quarter warp writes the eight columns of a 64-column slab's row.
         const int t = threadIdx.x - C::SM_WARPS * 32;
-        constexpr int SLABS = HD / 64;
-        const int j = t & 7, r = t >> 3;                    // piece of a slab's row, row of the group
-        const uint8_t* ksrc = static_cast<const uint8_t*>(a.kv.k) + (size_t)r * HD + 8 * j;
-        const uint8_t* vsrc = static_cast<const uint8_t*>(a.kv.v) + (size_t)r * HD + 8 * j;
-        const uint32_t to = r * 128 + ((j ^ (r & 7)) << 4);
-        // lane l: where group b0 + l lies in the pool, in groups (-1: nowhere), and its page in the next batch
-        auto place = [&](int g, int page) {
-            return g < g_stop && valid(page) ? ((page * NKV + h) << (lg - 4)) + (g & ((a.kv.page_size >> 4) - 1)) : -1;
+        constexpr int TPR = HD / 8, RPP = C::CV_WARPS * 32 / TPR, PASSES = 64 / RPP;
+        const int piece = t % TPR, r0 = t / TPR;
+        // where the 8 codes of row r lie in a box of codes (16-byte columns swizzled), and their f16 column
+        const int box = piece * 8 / C::COLS, c16 = (piece * 8 % C::COLS) >> 4;
+        auto from = [&](int r) {
+            const int x = C::COLS == 128 ? r & 7 : (r >> 1) & 3;
+            return box * (64 * C::COLS) + r * C::COLS + ((c16 ^ x) << 4) + (piece & 1) * 8;
         };
-        int b0 = j0 * C::GROUPS;
-        int here = place(b0 + lane, page_of(b0 + lane)), p1 = page_of(b0 + 32 + lane);
-        uint2 raw[C::GROUPS][SLABS];
-        auto fetch = [&](int e, int g0, int p) {            // group p of entry e, whose tile starts at lane g0
-            const int g = __shfl_sync(0xffffffffu, here, g0 + p);
-            const uint8_t* src = ((e & 1) ? vsrc : ksrc) + (size_t)(unsigned)g * (16 * HD);
-#pragma unroll
-            for (int i = 0; i < SLABS; i++) raw[p][i] = g >= 0 ? __ldg(reinterpret_cast<const uint2*>(src + 64 * i)) : make_uint2(0, 0);
-        };
-        if (n > 0) {
-#pragma unroll
-            for (int p = 0; p < C::GROUPS; p++) fetch(0, 0, p);
-        }
-        for (int e = 0; e < 2 * n; e++) {
+        auto to = [&](int r) { return (piece >> 3) * C::KBOX + r * 128 + (((piece & 7) ^ (r & 7)) << 4); };
+        bool ok = true;
+        for (int e = 0; e < 2 * n && ok; e++) {
             const int sl = e % C::NE;
-            if (e >= C::NE && !warp_wait(&empty[sl], ((e / C::NE) - 1) & 1, a.err, abort_flag)) break;
-            // the next entry's tile may start the next batch of groups (a batch is whole tiles)
-            int g0 = (j0 + ((e + 1) >> 1)) * C::GROUPS - b0;
-            if (g0 >= 32) {
-                b0 += 32;
-                g0 -= 32;
-                here = place(b0 + lane, p1);
-                p1 = page_of(b0 + 32 + lane);
-            }
-            uint8_t* dst = smem + C::OFF_RING + sl * C::KV_B + to;
-            const bool more = e + 1 < 2 * n;
+            if (e >= C::NE) ok = warp_wait(&empty[sl], ((e / C::NE) - 1) & 1, a.err, abort_flag);
+            uint8_t* dst = smem + C::OFF_RING + sl * C::KV_B;
 #pragma unroll
-            for (int p = 0; p < C::GROUPS; p++) {
+            for (int hf = 0; hf < C::HALVES; hf++) {
+                const int u = e * C::HALVES + hf, rs = u % C::NR;
+                ok = ok && warp_wait(&raw_full[rs], (u / C::NR) & 1, a.err, abort_flag);
+                if (!ok) break;
+                const uint8_t* src = smem + C::OFF_RAW + rs * C::RAW_B;
+                uint2 raw[PASSES];
 #pragma unroll
-                for (int i = 0; i < SLABS; i++) {
-                    const uint32_t x = raw[p][i].x ^ 0x80808080u, y = raw[p][i].y ^ 0x80808080u;
-                    *reinterpret_cast<uint4*>(dst + i * C::KBOX + p * 16 * 128) =
+                for (int p = 0; p < PASSES; p++) raw[p] = *reinterpret_cast<const uint2*>(src + from(r0 + p * RPP));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_empty[rs]);
+#pragma unroll
+                for (int p = 0; p < PASSES; p++) {
+                    const uint32_t x = raw[p].x ^ 0x80808080u, y = raw[p].y ^ 0x80808080u;
+                    *reinterpret_cast<uint4*>(dst + to(64 * hf + r0 + p * RPP)) =
                         make_uint4(code_pair(x, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4140), code_pair(y, 0x4342));
                 }
-                if (more) fetch(e + 1, g0, p);
             }
+            if (!ok) break;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[sl]);
         }
     } else {
-        if constexpr (C::SPLIT_REGS) regs_down<48>();
+        if constexpr (C::SPLIT_REGS) regs_down<72>();
         const int nu = __shfl_sync(0xffffffffu, n, 0), nq = __shfl_sync(0xffffffffu, nqt, 0);
-        if (warp == C::SM_WARPS + C::CV_WARPS && nu > 0) {
+        if (warp == C::SM_WARPS + C::CV_WARPS + 1) {
+            // ======================== TMA: a tile's codes as boxes of 16 keys, the smallest page; lane l holds the page of
+            // group b0 + l, and that of the next 32 groups
+            int b0 = j0 * C::GROUPS;
+            int p0 = page_of(b0 + lane), p1 = page_of(b0 + 32 + lane);
+            bool ok = true;
+            int e = 0;
+            for (; e < 2 * n * C::HALVES && ok; e++) {        // 64 keys of K or V: half h of entry e / HALVES
+                const int rs = e % C::NR;
+                if (e >= C::NR) ok = warp_wait(&raw_empty[rs], ((e / C::NR) - 1) & 1, a.err, abort_flag);
+                if (!ok) break;
+                const int ent = e / C::HALVES;
+                const int g = (j0 + (ent >> 1)) * C::GROUPS + 4 * (e % C::HALVES) + (lane & 3);
+                // K and V of a tile look up the same pages, so a tile is looked up from the batch it lies in
+                while (g - (lane & 3) - b0 >= 32) {
+                    b0 += 32;
+                    p0 = p1;
+                    p1 = page_of(b0 + 32 + lane);
+                }
+                const int page = __shfl_sync(0xffffffffu, p0, (g - b0) & 31);
+                const bool v = g < g_stop && valid(page);
+                const unsigned have = __ballot_sync(0xffffffffu, v && lane < 4);
+                if (lane == 0) mbar_arrive_expect_tx(&raw_full[rs], (uint32_t)(__popc(have) * 16 * HD));
+                __syncwarp();
+                if (v && lane < 4 * (HD / C::COLS)) {
+                    const int box = lane >> 2, y = ((page * NKV + h) << lg) + ((g << 4) & (a.kv.page_size - 1));
+                    tma_load_2d(smem + C::OFF_RAW + rs * C::RAW_B + box * (64 * C::COLS) + (lane & 3) * 16 * C::COLS,
+                                (ent & 1) ? &tmv : &tmk, box * C::COLS, y, &raw_full[rs]);
+                }
+            }
+            // no copy of this CTA may be in flight when it ends
+            for (int k = max(0, e - C::NR); k < e; k++) mbar_wait(&raw_full[k % C::NR], (k / C::NR) & 1, a.err);
+        } else if (warp == C::SM_WARPS + C::CV_WARPS && nu > 0) {
             // ======================== MMA issuer: the whole warp runs the loop and one elected lane issues, so that the
             // descriptors are uniform values (held per thread they had to be moved to uniform registers before each MMA:
             // 109 cycles between MMAs of 64)
@@ -591,7 +640,14 @@ cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
         return cudaFuncSetAttribute(paged_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_prefill_kernel<HD>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)), dim3(C::THREADS), (size_t)smem, st, a);
+    CUtensorMap tmk, tmv;
+    const uint64_t rows = (uint64_t)a.kv.n_pages * a.kv.n_kv_head * a.kv.page_size;
+    const CUtensorMapSwizzle swz = C::COLS == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    if (!encode_tmap_2d(&tmk, a.kv.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz) ||
+        !encode_tmap_2d(&tmv, a.kv.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz))
+        return cudaErrorInvalidValue;
+    return launch_pdl(paged_prefill_kernel<HD>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)), dim3(C::THREADS), (size_t)smem, st,
+                      tmk, tmv, a);
 }
 
 }  // namespace
