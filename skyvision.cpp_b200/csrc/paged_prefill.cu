@@ -33,7 +33,6 @@ namespace svkv {
 
 namespace {
 
-constexpr int kPolyOf4 = 0;               // exponentials of four that run on the FMA pipe
 constexpr float kSumLimit = 1024.0f;      // a row's sum over 64 keys against its m_r; p' stays below 4 of it
 constexpr float kVRefSlack = 2.0f;        // log2 vs may pass v_ref by this much before O is rescaled
 constexpr float kVFloor = -40.0f;         // log2 of the smallest vs / v_ref told apart (pages of zeros have vs = 0)
@@ -96,21 +95,6 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t r;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
     return r != 0;
-}
-
-// 2^x of two values on the FMA pipe: x = n + f, f in [-1/2, 1/2], 2^f by the polynomial that the f16-cache prefill uses
-// (degree 4, fitted for minimax relative error, 2.7e-6), n added into the exponent.  Below -126 it gives 2^-126 or
-// less (0 in f16); x is below 126 (kSumLimit is checked on the exponentials of the other pipe as well).
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    x = make_float2(fminf(fmaxf(x.x, -126.0f), 126.0f), fminf(fmaxf(x.y, -126.0f), 126.0f));
-    const float2 magic = make_float2(12582912.0f, 12582912.0f), minus = make_float2(-12582912.0f, -12582912.0f);
-    const float2 t = add2(x, magic), f = add2(x, mul2(add2(t, minus), make_float2(-1.0f, -1.0f)));
-    float2 p = fma2(make_float2(0.00956530869f, 0.00956530869f), f, make_float2(0.05591748655f, 0.05591748655f));
-    p = fma2(p, f, make_float2(0.2402486354f, 0.2402486354f));
-    p = fma2(p, f, make_float2(0.6931219101f, 0.6931219101f));
-    p = fma2(p, f, make_float2(0.9999992251f, 0.9999992251f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 template <int N>
@@ -207,27 +191,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
         const int pos = rq.z + tok;
         const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, hi = min(pos + 1, rq.w);
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(qtl * C::QCOLS);
-        {
-            const uint8_t* qrow = a.q + (size_t)(rq.x + tok) * a.q_nb;
-            uint8_t* qs = smem + qtl * C::Q_B;
-#pragma unroll 4
-            for (int e = 0; e < HD; e += 8) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (live) {
-                    if (a.q_type == SV_TYPE_F32) {
-                        const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qrow) + (size_t)hd * HD + e);
-                        const float4 f0 = f[0], f1 = f[1];
-                        v = make_uint4(pack_h2(f0.x, f0.y), pack_h2(f0.z, f0.w), pack_h2(f1.x, f1.y), pack_h2(f1.z, f1.w));
-                    } else {
-                        v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(qrow) + (size_t)hd * HD + e);
-                    }
-                }
-                *reinterpret_cast<uint4*>(qs + (e / 64) * C::QBOX + swz_off(r, e % 64, 128)) = v;
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
-        }
         // Scales of 32 groups at a time in this warp's own table: x = ks scale log2(e) (a page of zeros has zero
         // scores at any x > 0; a group without a page has x < 0), y = log2 vs - v_ref, z = 2^-y.
         float4* tab = reinterpret_cast<float4*>(smem + C::OFF_SC) + warp * 32;
@@ -243,6 +206,35 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
         int pg = page_of(j0 * C::GROUPS + lane);
         float2 next = scale_of(j0 * C::GROUPS + lane, pg);
         pg = page_of(j0 * C::GROUPS + 32 + lane);
+        {
+            const uint8_t* qrow = a.q + (size_t)(rq.x + tok) * a.q_nb;
+            uint8_t* qs = smem + qtl * C::Q_B;
+            constexpr int B = 16;                           // 16-byte columns in flight
+            for (int e0 = 0; e0 < HD; e0 += 8 * B) {
+                uint4 v[B];
+#pragma unroll
+                for (int k = 0; k < B; k++) {
+                    const int e = e0 + 8 * k;
+                    v[k] = make_uint4(0, 0, 0, 0);
+                    if (!live || e >= HD) continue;
+                    if (a.q_type == SV_TYPE_F32) {
+                        const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(qrow) + (size_t)hd * HD + e);
+                        const float4 f0 = f[0], f1 = f[1];
+                        v[k] = make_uint4(pack_h2(f0.x, f0.y), pack_h2(f0.z, f0.w), pack_h2(f1.x, f1.y), pack_h2(f1.z, f1.w));
+                    } else {
+                        v[k] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(qrow) + (size_t)hd * HD + e);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < B; k++) {
+                    const int e = e0 + 8 * k;
+                    if (e < HD) *reinterpret_cast<uint4*>(qs + (e / 64) * C::QBOX + swz_off(r, e % 64, 128)) = v[k];
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
         float m = -INFINITY, l = 0.0f, vref = -INFINITY;
         unsigned holes = 0;                                 // groups of the batch without a page
         bool ok = true;
@@ -298,7 +290,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
                         const float2 y = fma2(make_float2(x[16 * g + k], x[16 * g + k + 1]), c2, kk);
-                        const float2 p = (k / 2) % 4 < kPolyOf4 ? exp2_poly(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
                         s2 = add2(s2, p);
                         w[8 * g + k / 2] = pack_h2(p.x, p.y);
                     }
