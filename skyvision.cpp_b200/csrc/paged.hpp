@@ -8,7 +8,7 @@
 //   req       int4 per request: first row, rows, tokens held before, tokens held after
 //   page      int4 per page that the step writes to: first row, page, first offset, rows
 //   dec       two int4 per decode segment: request, its tiles [a, b), split | splits << 16; its req entry
-//   cta       first segment of each decode CTA (and one past the last)
+//   cta       first segment of each decode CTA (and one past the last); head_seg: a copy of that segment
 //   pre       int4 per prefill item: request, query tile, split, splits
 //   tickets   arrival counters of the split merges (zeroed by the plan, and again by each merge)
 //   *_part    unnormalised outputs of the splits; *_ml their running maximum and sum
@@ -32,7 +32,7 @@ constexpr int dec_ctas_per_sm(int hd, bool sixteen) { return (hd == 256 ? 2 : 3)
 constexpr int pre_rows(int hd) { return hd == 256 ? 128 : 256; }   // query rows of one prefill unit
 constexpr int pre_tile(int hd) { return hd == 256 ? 64 : 128; }    // keys per prefill tile
 // a split shorter than this costs more in its start and merge than it saves
-constexpr int kDecMinTiles = 4;
+constexpr int kDecMinTiles = 6;
 constexpr int kPreMinTiles = 4;
 
 enum : int { PH_PAGES = 0, PH_PRE = 1 };
@@ -41,7 +41,7 @@ struct StepLayout {
     int page_cap = 0, dec_cap = 0, pre_cap = 0;     // most entries of each list
     int few = kDecRows;                             // rows of a decode unit, at most
     int dec_slots = 1, pre_slots = 1;               // CTAs that run at once, per kv head
-    size_t head = 0, req = 0, page = 0, dec = 0, cta = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
+    size_t head = 0, req = 0, page = 0, dec = 0, cta = 0, head_seg = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
     size_t bytes = 0;
     int n_ticks = 0;
 };

@@ -87,8 +87,10 @@ struct Seg {
     int4 rq;                     // first row, rows, keys held before, after
 };
 
-__device__ __forceinline__ Seg seg_of(const PagedAttn& a, int i) {
-    const int4* d = reinterpret_cast<const int4*>(a.work + a.l.dec) + 2 * (size_t)i;
+// Segment i; a CTA's first is read from the copy that lies by the CTA's own number, beside its range
+__device__ __forceinline__ Seg seg_of(const PagedAttn& a, int i, int first_of = -1) {
+    const int4* d = first_of < 0 ? reinterpret_cast<const int4*>(a.work + a.l.dec) + 2 * (size_t)i
+                                 : reinterpret_cast<const int4*>(a.work + a.l.head_seg) + 2 * (size_t)first_of;
     const int4 x = __ldg(d);
     Seg s;
     s.rq = __ldg(d + 1);
@@ -167,8 +169,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         Seg s;
         int p1 = -1;
         Batch b0, b1;
+        s = seg_of(a, g0, cta);                                   // (stale where the CTA has none: not used)
         if (g0 < g1) {
-            s = seg_of(a, g0);
             b0 = batch_of(page_of(s, 4 * s.j0 + lane));
             p1 = page_of(s, 4 * s.j0 + 32 + lane);
         }
@@ -231,7 +233,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     const int c0 = 2 * tq, c1 = (2 * tq + 1) ^ 4;              // keys of MMA indexes 2 tq, 2 tq + 1
     int tile = 0;
     for (int sg = g0; sg < g1; sg++) {
-        const Seg sgm = seg_of(a, sg);
+        const Seg sgm = seg_of(a, sg, sg == g0 ? cta : -1);
         const int4 rq = sgm.rq;
         const int rows = rq.y * a.G, n = sgm.j1 - sgm.j0;
         // Q^T fragments: row gq (of each row tile), bytes 16 tq.. of each 64-dim group over four k-steps
@@ -519,18 +521,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             float M = -INFINITY, L = 0.0f;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s0 = 0; s0 < ns; s0 += 8) {                       // eight segments' loads in flight
-                float2 ml[8];
-                float4 y[8];
+            constexpr int U = 16;                                      // segments whose loads are in flight
+            for (int s0 = 0; s0 < ns; s0 += U) {
+                float2 ml[U];
+                float4 y[U];
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
+                for (int u = 0; u < U; u++) {
                     const int s = min(s0 + u, ns - 1);
                     ml[u] = __ldcg(pml + s * sm + r);
                     y[u] = __ldcg(reinterpret_cast<const float4*>(po + s * so + (size_t)r * HD + d));
                 }
                 float mn = M;
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
+                for (int u = 0; u < U; u++) {
                     if (s0 + u >= ns) ml[u] = make_float2(-INFINITY, 0.0f);
                     mn = fmaxf(mn, ml[u].x);
                 }
@@ -540,7 +543,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 L *= g;
                 x.x *= g; x.y *= g; x.z *= g; x.w *= g;
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
+                for (int u = 0; u < U; u++) {
                     const float f = ml[u].x == -INFINITY ? 0.0f : fast_exp2(ml[u].x - mn);
                     L = fmaf(f, ml[u].y, L);
                     x.x = fmaf(f, y[u].x, x.x); x.y = fmaf(f, y[u].y, x.y); x.z = fmaf(f, y[u].z, x.z); x.w = fmaf(f, y[u].w, x.w);

@@ -16,7 +16,6 @@ namespace svkv {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kRowsPerBlock = 512;
 
 struct PlanArgs {
@@ -28,7 +27,7 @@ struct PlanArgs {
 };
 
 // exclusive prefix sum over the block's threads; *total gets the sum
-template <class T>
+template <int kThreads, class T>
 __device__ __forceinline__ T block_scan(T x, T* total, T* buf) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     T v = x;
@@ -61,30 +60,35 @@ __device__ __forceinline__ int find_last(const int* start, int n, int x) {
     return lo;
 }
 
-// Splits of units so that their items fill `slots` once: the shortest piece length (in tiles) that gives
-// no more than `slots` items, but at least min_tiles.  cost(u): tiles of unit u (0: not a unit).
-template <class Cost>
+// Piece length (in tiles) for units of cost(u) tiles each.  Up to `slots` units: the shortest that gives no more than
+// `slots` items, so all run at once.  Up to kMoreWaves times as many: pieces of a kMoreWaves-th of an even share, so that the last
+// wave is short.  More units than that: whole units.  At least min_tiles in any case.
+constexpr int kMoreWaves = 3;
+template <int kThreads, class Cost>
 __device__ int piece_of(int n_units, int slots, int min_tiles, Cost cost, long long* buf) {
+    if (n_units > kMoreWaves * slots) return INT32_MAX;
     long long sum = 0, total;
     for (int u = threadIdx.x; u < n_units; u += kThreads) sum += cost(u);
-    block_scan<long long>(sum, &total, buf);
+    block_scan<kThreads, long long>(sum, &total, buf);
+    if (n_units > slots) {
+        const long long share = (total + kMoreWaves * slots - 1) / (kMoreWaves * slots);
+        return (int)(share > min_tiles ? share : min_tiles);
+    }
     long long piece = (total + slots - 1) / slots;
     if (piece < min_tiles) piece = min_tiles;
     for (int it = 0; it < 8; it++) {
-        long long n = 0, all;
-        for (int u = threadIdx.x; u < n_units; u += kThreads) n += (cost(u) + piece - 1) / piece;
-        block_scan<long long>(n, &all, buf);
+        int n = 0, all;
+        for (int u = threadIdx.x; u < n_units; u += kThreads) n += (int)((cost(u) + piece - 1) / piece);
+        block_scan<kThreads, int>(n, &all, reinterpret_cast<int*>(buf));
         if (all <= slots) break;
         const long long next = (piece * all + slots - 1) / slots;
-        if (next >= total) {
-            piece = total > min_tiles ? total : min_tiles;
-            break;
-        }
         piece = next > piece ? next : piece + 1;
     }
-    return (int)piece;
+    return (int)(piece < INT32_MAX ? piece : INT32_MAX);
 }
 
+// kThreads: 128 for a few requests (shorter barriers), 512 otherwise
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_constant__ PlanArgs a) {
     extern __shared__ int sm[];
     __shared__ long long buf[kThreads / 32];
@@ -96,6 +100,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
     int* touched = taken + n + 1;      // [n + 1] pages written to before r
     int* tiles = touched + n + 1;      // [n + 1] prefill query tiles before r
     pdl_wait();
+    if (threadIdx.x == 0) pdl_trigger();
     const int per = (n + kThreads - 1) / kThreads;
     const int r0 = min(n, (int)threadIdx.x * per), r1 = min(n, r0 + per);
     const int nf = min(max(__ldg(a.n_free), 0), s.n_pages);
@@ -111,7 +116,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
             sum += c;
         }
         long long total;
-        long long at = block_scan<long long>(sum, &total, buf);
+        long long at = block_scan<kThreads, long long>(sum, &total, buf);
         for (int r = r0; r < r1; r++) {
             const int c = start[r];
             start[r] = (int)min(at, (long long)s.n_tokens);
@@ -126,35 +131,34 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
         // pages taken and pages touched are below 2^31 each: scanned as the two halves of one word
         unsigned long long sum = 0;
         int tl = 0;
-        auto of = [&](int r, int* np, int* nt, int* ql) {
+        auto of = [&](int r, int* ql) {
             const int p = past[r], c = start[r + 1] - start[r];
             const int held = (p + ps - 1) >> lg, want = min((p + c + ps - 1) >> lg, s.max_blocks);
-            *np = max(want - held, 0);
-            *nt = c > 0 ? ((p + c - 1) >> lg) - (p >> lg) + 1 : 0;
             *ql = c * a.G > a.l.few ? (c * a.G + rows_per_unit - 1) / rows_per_unit : 0;
+            return ((unsigned long long)max(want - held, 0) << 32) | (unsigned)(c > 0 ? ((p + c - 1) >> lg) - (p >> lg) + 1 : 0);
         };
         for (int r = r0; r < r1; r++) {
-            int np, nt, ql;
-            of(r, &np, &nt, &ql);
-            sum += ((unsigned long long)np << 32) | (unsigned)nt;
+            int ql;
+            sum += of(r, &ql);
             tl += ql;
         }
         unsigned long long total;
-        unsigned long long at = block_scan<unsigned long long>(sum, &total, reinterpret_cast<unsigned long long*>(buf));
-        long long ttl, tat = block_scan<long long>(tl, &ttl, buf);
+        unsigned long long at = block_scan<kThreads, unsigned long long>(sum, &total, reinterpret_cast<unsigned long long*>(buf));
+        int ttl = 0, tat = 0;
+        if (blockIdx.x == 0 && a.l.pre_cap > 0) tat = block_scan<kThreads, int>(tl, &ttl, reinterpret_cast<int*>(buf));
         for (int r = r0; r < r1; r++) {
-            int np, nt, ql;
-            of(r, &np, &nt, &ql);
+            int ql;
+            const unsigned long long x = of(r, &ql);
             taken[r] = (int)(at >> 32);
             touched[r] = (int)(at & 0xffffffffu);
-            tiles[r] = (int)tat;
-            at += ((unsigned long long)np << 32) | (unsigned)nt;
+            tiles[r] = tat;
+            at += x;
             tat += ql;
         }
         if (threadIdx.x == 0) {
             taken[n] = (int)(total >> 32);
             touched[n] = (int)(total & 0xffffffffu);
-            tiles[n] = (int)ttl;
+            tiles[n] = ttl;
         }
     }
     __syncthreads();
@@ -216,38 +220,47 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
         // piece's part of a request is a segment
         int4* dec = reinterpret_cast<int4*>(work + a.l.dec);
         int* cta = reinterpret_cast<int*>(work + a.l.cta);
+        int4* head_seg = reinterpret_cast<int4*>(work + a.l.head_seg);
         auto dec_cost = [&](int r) {
             const int c = start[r + 1] - start[r];
             if (c == 0 || c * a.G > a.l.few) return 0;
             return (past[r] + c + kDecTile - 1) / kDecTile;
         };
         if (a.l.dec_cap > 0) {
-            long long line;
-            {
-                long long sum = 0;
+            // all counts below 2^31: the step's layout bounds requests x table rows
+            int line = 0;
+            const bool one = n <= kThreads;                // one request per thread: the line's scan tells its length
+            if (!one) {
+                int sum = 0;
                 for (int r = threadIdx.x; r < n; r += kThreads) sum += dec_cost(r);
-                block_scan<long long>(sum, &line, buf);
+                block_scan<kThreads, int>(sum, &line, reinterpret_cast<int*>(buf));
             }
-            const long long even = (line + a.l.dec_slots - 1) / a.l.dec_slots;
-            const long long piece = even < kDecMinTiles ? kDecMinTiles : even;
-            long long t0 = 0;
-            int base = 0;
+            int t0 = 0, base = 0, piece = 0;
             for (int u0 = 0; u0 < n; u0 += kThreads) {
                 const int r = u0 + threadIdx.x;
-                const long long c = r < n ? dec_cost(r) : 0;
-                long long all, t = t0 + block_scan<long long>(c, &all, buf);
+                const int c = r < n ? dec_cost(r) : 0;
+                int all, segs;
+                const int t = t0 + block_scan<kThreads, int>(c, &all, reinterpret_cast<int*>(buf));
                 t0 += all;
-                const int ns = c > 0 ? (int)((t + c - 1) / piece - t / piece) + 1 : 0;
-                const int at = base + (int)block_scan<long long>(ns, &all, buf);
-                base += (int)all;
+                if (one) line = all;
+                if (u0 == 0) piece = max((line + a.l.dec_slots - 1) / a.l.dec_slots, kDecMinTiles);
+                const int p0 = t / piece, ns = c > 0 ? (t + c - 1) / piece - p0 + 1 : 0;
+                const int at = base + block_scan<kThreads, int>(ns, &segs, reinterpret_cast<int*>(buf));
+                base += segs;
+                const int4 q = ns > 0 ? req_of(r) : make_int4(0, 0, 0, 0);
                 for (int i = 0; i < ns; i++) {
-                    const long long lo = (t / piece + i) * piece, g0 = lo > t ? lo : t, g1 = lo + piece < t + c ? lo + piece : t + c;
-                    dec[2 * (at + i)] = make_int4(r, (int)(g0 - t), (int)(g1 - t), i | ns << 16);
-                    dec[2 * (at + i) + 1] = req_of(r);
-                    if (g0 == lo) cta[lo / piece] = at + i;
+                    const int lo = (p0 + i) * piece, g0 = max(lo, t), g1 = (int)min((long long)lo + piece, (long long)t + c);
+                    const int4 x = make_int4(r, g0 - t, g1 - t, i | ns << 16);
+                    dec[2 * (at + i)] = x;
+                    dec[2 * (at + i) + 1] = q;
+                    if (g0 == lo) {                        // the piece's first segment: where its CTA looks first
+                        cta[p0 + i] = at + i;
+                        head_seg[2 * (p0 + i)] = x;
+                        head_seg[2 * (p0 + i) + 1] = q;
+                    }
                 }
             }
-            for (long long i = (line + piece - 1) / piece + threadIdx.x; i <= a.l.dec_slots; i += kThreads) cta[i] = base;
+            for (int i = (line + piece - 1) / piece + threadIdx.x; i <= a.l.dec_slots; i += kThreads) cta[i] = base;
         }
         // ---- prefill items: query tiles of the other requests, last ones (most keys) first
         int4* pre = reinterpret_cast<int4*>(work + a.l.pre);
@@ -260,16 +273,16 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
         };
         int pbase = 0;
         if (n_tiles > 0) {
-            const int piece = piece_of(n_tiles, a.l.pre_slots, kPreMinTiles, pre_cost, buf);
+            const int piece = piece_of<kThreads>(n_tiles, a.l.pre_slots, kPreMinTiles, pre_cost, buf);
             for (int u0 = 0; u0 < n_tiles; u0 += kThreads) {
                 const int u = n_tiles - 1 - (u0 + (int)threadIdx.x);
-                const int ns = u >= 0 ? (pre_cost(u) + piece - 1) / piece : 0;
-                long long all, at = block_scan<long long>(ns, &all, buf);
+                const int ns = u >= 0 ? (int)(((long long)pre_cost(u) + piece - 1) / piece) : 0;
+                int all, at = block_scan<kThreads, int>(ns, &all, reinterpret_cast<int*>(buf));
                 if (u >= 0) {
                     const int r = tile_req(u);
                     for (int i = 0; i < ns; i++) pre[pbase + at + i] = make_int4(r, u - tiles[r], i, ns);
                 }
-                pbase += (int)all;
+                pbase += all;
             }
         }
         if (threadIdx.x == 0) {
@@ -281,17 +294,19 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
     if (err && s.err) atomicOr(s.err, err);
 }
 
+constexpr int kReleaseThreads = 256;
+
 // One block: the pages of the n requests go back in order (exclusive prefix sum of their page counts).
-__global__ void __launch_bounds__(kThreads) paged_release_kernel(int32_t* table, int n_req, int max_blocks, int lg,
+__global__ void __launch_bounds__(kReleaseThreads) paged_release_kernel(int32_t* table, int n_req, int max_blocks, int lg,
                                                                  int n_pages, const int32_t* req, int n,
                                                                  const int32_t* kv_len, int32_t* free_pages,
                                                                  int32_t* n_free, int* err) {
-    __shared__ long long buf[kThreads / 32];
+    __shared__ long long buf[kReleaseThreads / 32];
     pdl_wait();
     long long at0 = max(__ldg(n_free), 0);
     int bad = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += kThreads) {
+    for (int i0 = 0; i0 < n; i0 += kReleaseThreads) {
         const int i = i0 + threadIdx.x;
         int r = -1, blocks = 0;
         if (i < n) {
@@ -299,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) paged_release_kernel(int32_t* table,
             if (r < 0 || r >= n_req) bad |= SV_DEVERR_STEP;
             else blocks = (int)min(((long long)max(__ldg(kv_len + i), 0) + (1 << lg) - 1) >> lg, (long long)max_blocks);
         }
-        long long all, at = at0 + block_scan<long long>(blocks, &all, buf);
+        long long all, at = at0 + block_scan<kReleaseThreads, long long>(blocks, &all, buf);
         for (int j = 0; j < blocks; j++, at++) {
             int32_t* e = table + (size_t)r * max_blocks + j;
             if (at < n_pages) free_pages[at] = *e;
@@ -324,6 +339,8 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     if (s.head_dim != 64 && s.head_dim != 128 && s.head_dim != 256) return false;
     if (s.n_kv_head < 1 || s.n_head < 1 || s.n_head % s.n_kv_head != 0) return false;
     // rows of the pool, positions and row x head products stay in 31 bits
+    // (and the key tiles of all requests, 64 keys each)
+    if ((int64_t)s.n_req * s.max_blocks * (ps / 16) / 4 > INT32_MAX / 4) return false;
     if (s.n_kv_head > 1024 || (int64_t)s.n_pages * ps * s.n_kv_head > INT32_MAX || (int64_t)s.max_blocks * ps > INT32_MAX / 2 ||
         (int64_t)s.n_tokens * s.n_head > INT32_MAX)
         return false;
@@ -339,7 +356,7 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     const int rows = pre_rows(s.head_dim);
     if ((int64_t)max_new * G > l->few) {
         const int64_t least = l->few / G + 1;    // fewest tokens of a prefill request
-        l->pre_cap = (int)(T * G / rows + (act < T / least ? act : T / least) + l->pre_slots);
+        l->pre_cap = (int)(T * G / rows + (act < T / least ? act : T / least) + kMoreWaves * l->pre_slots);
     }
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -353,6 +370,7 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     l->page = take(sizeof(int4) * (size_t)l->page_cap);
     l->dec = take(2 * sizeof(int4) * (size_t)l->dec_cap);
     l->cta = take(sizeof(int) * (size_t)(l->dec_slots + 1));
+    l->head_seg = take(2 * sizeof(int4) * (size_t)(l->dec_cap ? l->dec_slots : 0));
     l->pre = take(sizeof(int4) * (size_t)l->pre_cap);
     l->tick = take(sizeof(int) * (size_t)l->n_ticks);
     l->dec_part = take(sizeof(float) * (size_t)l->dec_cap * s.n_kv_head * kDecRows * s.head_dim);
@@ -370,17 +388,19 @@ cudaError_t launch_paged_plan(const sv_paged_step& s, const StepLayout& l, const
     static std::once_flag once[kMaxDevices];
     static cudaError_t status[kMaxDevices];
     const cudaError_t e = once_per_device(once, status, [] {
-        return cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(paged_plan_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     (5 * SV_PAGED_MAX_REQ + 4) * (int)sizeof(int));
     });
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_plan_kernel, dim3(1 + ceil_div(s.n_tokens, kRowsPerBlock)), dim3(kThreads), smem, st, a);
+    const dim3 grid(1 + ceil_div(s.n_tokens, kRowsPerBlock));
+    return s.n_req <= 128 ? launch_pdl(paged_plan_kernel<128>, grid, dim3(128), smem, st, a)
+                          : launch_pdl(paged_plan_kernel<512>, grid, dim3(512), smem, st, a);
 }
 
 cudaError_t launch_paged_release(int32_t* table, int n_req, int max_blocks, int ps, int n_pages, const int32_t* req,
                                  int n, const int32_t* kv_len, int32_t* free_pages, int32_t* n_free, int* err,
                                  cudaStream_t st) {
-    return launch_pdl(paged_release_kernel, dim3(1), dim3(kThreads), 0, st, table, n_req, max_blocks, log2_of(ps),
+    return launch_pdl(paged_release_kernel, dim3(1), dim3(kReleaseThreads), 0, st, table, n_req, max_blocks, log2_of(ps),
                       n_pages, req, n, kv_len, free_pages, n_free, err);
 }
 
