@@ -20,9 +20,9 @@
 // shared load then hit eight different 16-byte columns for K and for V.
 //
 // The running maximum is lazy: a row's reference m_r moves only when a score passes it by 2^8, found by
-// a vote, so a tile normally needs no shuffle and no rescaling; p <= 2^8 is far inside f16.  P is rounded to f16
-// for the second product (2^-12 relative on average, like the f16 output itself); sums stay f32.  P also
-// carries vs / v_ref, where v_ref trails the largest vs seen by at most 4.
+// a vote, so a tile normally needs no shuffle and no rescaling; p <= 2^8 is far inside f16.  P enters the second product
+// as two f16 parts (22 bits: with one, few rows' outputs were up to 1.6 times as far off as their own rounding); sums
+// stay f32.  P also carries vs / v_ref, where v_ref trails the largest vs seen by at most 4.
 // The warps of a CTA meet pairwise in shared memory.  Segments of one request and head meet in the work space; the
 // last to arrive (a ticket) adds them in order, so results do not depend on which one that is.
 //
@@ -359,7 +359,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                     }
                 }
                 const float pv = s2.y * vinv;
-                uint32_t pb[NT][2];
+                uint32_t pb[NT][2], pl[NT][2];                 // P as f16, and what that leaves of it
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
                     float p[4];
@@ -370,8 +370,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                     }
                     l[r][0] += p[0] + p[2];
                     l[r][1] += p[1] + p[3];
-                    pb[r][0] = movm_t(pack_h2(p[0] * pv, p[1] * pv));
-                    pb[r][1] = movm_t(pack_h2(p[2] * pv, p[3] * pv));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float x = p[2 * e] * pv, y = p[2 * e + 1] * pv;
+                        const __half2 hp = __floats2half2_rn(x, y);
+                        const float2 back = __half22float2(hp);
+                        pb[r][e] = movm_t(*reinterpret_cast<const uint32_t*>(&hp));
+                        pl[r][e] = movm_t(pack_h2(x - back.x, y - back.y));
+                    }
                 }
                 // V: 16 bytes (8 at HD 64) of keys c0, c1, 8 + c0, 8 + c1
                 constexpr int VB = HD >= 128 ? 16 : 8;
@@ -399,8 +405,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                             const uint32_t x = prmt(u0, u1, d ? 0x7362 : 0x5140), y = prmt(u2, u3, d ? 0x7362 : 0x5140);
                             const uint32_t f[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
 #pragma unroll
-                            for (int r = 0; r < NT; r++)
+                            for (int r = 0; r < NT; r++) {
                                 mma_f16(o[slab * (VB / 2) + 2 * j + d][r], f, pb[r][0], pb[r][1]);
+                                mma_f16(o[slab * (VB / 2) + 2 * j + d][r], f, pl[r][0], pl[r][1]);
+                            }
                         }
                     }
                 }

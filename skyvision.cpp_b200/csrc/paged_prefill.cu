@@ -5,7 +5,7 @@
 //   o_r  = sum_j p_rj vs[page(j)] c'_j / sum_j p_rj
 // The scales belong to a page and head, so both products run on the codes alone, which are exact in f16: one MMA
 // part per tile where a block-scaled row format needs two.  ks is applied to finished scores, vs / v_ref to the
-// weights before they are rounded to f16 (2^-12 relative on average, like an f16 output); sums stay f32.
+// weights before they are rounded to f16 (see kTwoPartRows); sums stay f32.
 //
 // Work item (from the plan): NQT tiles of 128 rows of one request and kv head (rows = tokens x the G query
 // heads, packed, so any G fills them) x a piece of the keys they see.  Roles:
@@ -34,6 +34,11 @@ namespace svkv {
 namespace {
 
 constexpr float kSumLimit = 1024.0f;      // a row's sum over 64 keys against its m_r; p' stays below 4 of it
+// Steps of up to this many query rows (tokens x heads) give P to the tensor core as two f16 parts (TWO).  One part costs
+// ~2.1e-4 of the output's norm, as much as an f16 output's own rounding, so together 1.41 times the latter; over few rows that
+// scatters (up to 1.6 times seen in steps of 160 to 8192 rows, 1.47 in larger ones).  The second part costs 13 to 35 % of
+// the time (512 rows x 16 heads of 256: 74 -> 84 us; 8192 x 32 of 128: 1.77 -> 2.39 ms).
+constexpr int kTwoPartRows = 8192;
 constexpr float kVRefSlack = 2.0f;        // log2 vs may pass v_ref by this much before O is rescaled
 constexpr float kVFloor = -40.0f;         // log2 of the smallest vs / v_ref told apart (pages of zeros have vs = 0)
 
@@ -102,7 +107,7 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <int HD>
+template <int HD, bool TWO>
 __global__ void __launch_bounds__(PreCfgP<HD>::THREADS, 1)
 paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                      const __grid_constant__ PagedAttn a) {
@@ -270,7 +275,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
             // 32 columns at a time: the next are on their way from TMEM while these become weights
             constexpr int CH = C::BN / 32;
             float s[2][32];
-            uint32_t pk[32];
+            uint32_t pk[32], pl[TWO ? 32 : 1];              // P as f16, and what that leaves of it
             float sum = 0.0f;
             auto mask = [&](float* x, int c) {              // this row's visible keys of 32
                 const int a0 = lo - kb - 32 * c, a1 = hi - kb - 32 * c;
@@ -279,7 +284,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                 for (int k = 0; k < 32; k++)
                     if (k < a0 || k >= a1 || ((hole >> (k / 16)) & 1)) x[k] = -INFINITY;
             };
-            auto weights = [&](const float* x, int c, uint32_t* w) {
+            auto weights = [&](const float* x, int c, uint32_t* w, uint32_t* wl) {
                 const float mneg = m == -INFINITY ? 0.0f : -m;
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
@@ -292,7 +297,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                         const float2 y = fma2(make_float2(x[16 * g + k], x[16 * g + k + 1]), c2, kk);
                         const float2 p = make_float2(fast_exp2(y.x), fast_exp2(y.y));
                         s2 = add2(s2, p);
-                        w[8 * g + k / 2] = pack_h2(p.x, p.y);
+                        if constexpr (TWO) {                // the upper 11 bits are exact in f16, the rest goes with them
+                            const float2 up = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xffffe000u),
+                                                          __uint_as_float(__float_as_uint(p.y) & 0xffffe000u));
+                            w[8 * g + k / 2] = pack_h2(up.x, up.y);
+                            wl[8 * g + k / 2] = pack_h2(p.x - up.x, p.y - up.y);
+                        } else {
+                            w[8 * g + k / 2] = pack_h2(p.x, p.y);
+                        }
                     }
                     sum = fmaf(s2.x + s2.y, t.z, sum);
                 }
@@ -304,7 +316,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                 const int hf = c / 2;
                 if (c + 1 < CH) tmem_ld32(sbuf + 32 * (c + 1), s[(c + 1) & 1]);
                 if (edge) mask(s[c & 1], c);
-                weights(s[c & 1], c, pk + 16 * (c & 1));
+                weights(s[c & 1], c, pk + 16 * (c & 1), pl + (TWO ? 16 * (c & 1) : 0));
                 if (c & 1) {
                     if (__any_sync(0xffffffffu, !(sum <= kSumLimit) || m == -INFINITY) || (hf == 0 && vmove != 1.0f)) {
                         // the rows' maxima over this half, O and the sums to match, and the half once more
@@ -346,12 +358,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                             tmem_ld32(sbuf + 64 * hf + 32 * k, t);
                             tmem_wait_ld();
                             if (edge) mask(t, 2 * hf + k);
-                            weights(t, 2 * hf + k, pk + 16 * k);
+                            weights(t, 2 * hf + k, pk + 16 * k, pl + (TWO ? 16 * k : 0));
                         }
                     }
                     l += sum;
                     sum = 0.0f;
-                    tmem_st32(sbuf + 32 * hf, reinterpret_cast<const float*>(pk));
+                    tmem_st32(sbuf + 64 * hf, reinterpret_cast<const float*>(pk));     // over the half's own columns
+                    if constexpr (TWO) tmem_st32(sbuf + 64 * hf + 32, reinterpret_cast<const float*>(pl));
                 }
                 // P is announced a chunk after it was stored (the last at once): the store is done by then
                 if ((c & 1) == 0 ? c > 0 : c + 1 == CH) {
@@ -579,8 +592,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                     tc_fence_after();
                     if (lead) {
 #pragma unroll
-                        for (int kk = 4 * hf; kk < 4 * hf + 4; kk++)
-                            umma_f16_ts(o, p + kk * 8, vd + (uint32_t)(kk * 16 * 128 >> 4), hi, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < 4; kk++)
+                            umma_f16_ts(o, p + 64 * hf + kk * 8, vd + (uint32_t)((4 * hf + kk) * 16 * 128 >> 4), hi, idesc_o,
+                                        (i > 0 || hf > 0 || kk > 0) ? 1u : 0u);
+                        if constexpr (TWO) {
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++)
+                                umma_f16_ts(o, p + 64 * hf + 32 + kk * 8, vd + (uint32_t)((4 * hf + kk) * 16 * 128 >> 4), hi, idesc_o, 1u);
+                        }
                         umma_commit(hf + 1 < C::HALVES ? &o_half[q] : &o_done[2 * q + (i & 1)]);
                     }
                     __syncwarp();
@@ -622,14 +641,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
     }
 }
 
-template <int HD>
-cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
+template <int HD, bool TWO>
+cudaError_t launch_parts(const PagedAttn& a, cudaStream_t st) {
     using C = PreCfgP<HD>;
     constexpr int smem = C::SMEM + 1024;
     static std::once_flag once[kMaxDevices];
     static cudaError_t status[kMaxDevices];
     const cudaError_t e = once_per_device(once, status, [] {
-        return cudaFuncSetAttribute(paged_prefill_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return cudaFuncSetAttribute(paged_prefill_kernel<HD, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
     if (e != cudaSuccess) return e;
     CUtensorMap tmk, tmv;
@@ -638,8 +657,13 @@ cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
     if (!encode_tmap_2d(&tmk, a.kv.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz) ||
         !encode_tmap_2d(&tmv, a.kv.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz))
         return cudaErrorInvalidValue;
-    return launch_pdl(paged_prefill_kernel<HD>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)), dim3(C::THREADS), (size_t)smem, st,
+    return launch_pdl(paged_prefill_kernel<HD, TWO>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)), dim3(C::THREADS), (size_t)smem, st,
                       tmk, tmv, a);
+}
+
+template <int HD>
+cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
+    return (int64_t)a.n_tokens * a.n_head <= kTwoPartRows ? launch_parts<HD, true>(a, st) : launch_parts<HD, false>(a, st);
 }
 
 }  // namespace
