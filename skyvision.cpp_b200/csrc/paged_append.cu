@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(256, NV == 1 ? 3 : 2) paged_append_few(const _
 
 // ---------------- up to NV x (THREADS / C) rows per page; K, V and the queries in blocks of their own
 template <int HD, bool F32, int ROT, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 3 : 2) paged_append_many(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : NV <= 2 ? 4 : 2) paged_append_many(const __grid_constant__ AppendArgs a) {
     constexpr int C = HD / 8, RP = THREADS / C;    // threads per row, rows per pass
     constexpr int ES = F32 ? 4 : 2, W = THREADS / 32;
     extern __shared__ __align__(16) float cs[];
