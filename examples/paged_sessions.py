@@ -1,0 +1,165 @@
+"""Sessions over the paged 8-bit cache, the way a server runs them.
+
+A fixed number of seats shares one pool of pages.  Prompts of unlike lengths come in as one step (plan, then in
+every layer rope_append and attn), then all seats decode one token a step as replays of one captured graph: the
+lengths, tables and the free list live on the device and nothing is read back in between.  At the end some
+sessions leave, their pages go back to the free list, and new prompts take them while the others decode on.
+
+The decoder is a stand-in (random projections around the attention).  The printed error compares the first
+layer's last attention with a 64-bit attention over the rows as they were before they became 8-bit codes.
+
+    python examples/paged_sessions.py [--seats 8] [--prompt 700] [--tokens 64] [--layers 4]
+"""
+import argparse
+import os
+import sys
+
+import numpy as np
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from __graft_entry__ import load_package  # noqa: E402
+
+sv = load_package()
+
+
+class Server:
+    def __init__(self, seats, n_layer, n_head, n_kv, hd, page_size, n_pages, max_len, max_rows, device=0):
+        dev = self.dev = torch.device("cuda", device)
+        self.kv = sv.PagedKv(n_layer, n_kv, hd, page_size, n_pages, device)
+        self.prompt_step = sv.PagedStep(seats, max_rows, max_rows, page_size, n_pages, n_head, n_kv, hd, device)
+        self.token_step = sv.PagedStep(seats, seats, 1, page_size, n_pages, n_head, n_kv, hd, device)
+        self.rope = sv.Rope(hd, freq_base=10000.0)
+        ints = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+        self.held, self.new = ints(seats), ints(seats)
+        self.table = ints(seats, -(-max_len // page_size)) - 1
+        self.free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
+        self.seats, self.n_head, self.n_kv, self.hd = seats, n_head, n_kv, hd
+        d = n_head * hd
+        g = torch.Generator(device=dev).manual_seed(1)
+        w = lambda *s: (torch.randn(s, generator=g, device=dev) / np.sqrt(s[0])).half()  # noqa: E731
+        self.layers = [(w(d, d + 2 * n_kv * hd), w(d, d), torch.ones(hd, device=dev), torch.ones(hd, device=dev))
+                       for _ in range(n_layer)]
+        self.first = None                # the first layer's (k, v, q, attention) of the step
+
+    def forward(self, step, x):
+        """One step of every layer: x [rows, d] -> [rows, d].  held and new say whose rows they are."""
+        h, kvh, hd = self.n_head, self.n_kv, self.hd
+        step.plan(self.held, self.new, self.table, self.free, self.n_free)
+        for i, (w_qkv, w_o, qn, kn) in enumerate(self.layers):
+            rows = torch.nn.functional.rms_norm(x, x.shape[1:]).matmul(w_qkv).view(-1, h + 2 * kvh, hd)
+            k, v = rows[:, h:h + kvh], rows[:, h + kvh:]
+            q = self.kv.rope_append(i, step, rows[:, :h], k, v, rope=self.rope, q_norm=qn, k_norm=kn)
+            a = self.kv.attn(i, step, q, 1 / np.sqrt(hd))
+            if i == 0:
+                self.first = (k, v, q, a)
+            x = x + a.view(x.shape).matmul(w_o)
+        self.n_free.copy_(step.n_free)
+        self.held.copy_(step.kv_len)
+        return x
+
+    def leave(self, seats):
+        """These sessions end: their pages go back to the free list."""
+        req = torch.tensor(seats, dtype=torch.int32, device=self.dev)
+        self.kv.release(self.table, req, self.held[req.long()], self.free, self.n_free)
+        self.held[req.long()] = 0
+
+    def check(self):
+        for flags in (self.kv.error_flags(), self.prompt_step.error_flags(), self.token_step.error_flags()):
+            if flags:
+                raise RuntimeError(f"device error flags {flags}")
+
+
+def rotated(k, pos, base=10000.0):
+    """[n, heads, hd] normed and rotated in 64 bits"""
+    k = k.double().cpu().numpy()
+    k = k / np.sqrt((k * k).mean(-1, keepdims=True) + 1e-6)
+    half = k.shape[-1] // 2
+    a = np.asarray(pos)[:, None] * base ** (-np.arange(half) / half)
+    c, s = np.cos(a)[:, None], np.sin(a)[:, None]
+    return np.concatenate([k[..., :half] * c - k[..., half:] * s, k[..., :half] * s + k[..., half:] * c], -1)
+
+
+def run(seats=8, prompt=700, tokens=64, layers=4, n_head=16, n_kv=4, hd=128, page_size=32):
+    rng = np.random.default_rng(0)
+    lens = rng.integers(max(1, prompt // 4), prompt + 1, seats)
+    max_len = prompt + 2 * tokens + 1
+    n_pages = seats * -(-max_len // page_size)
+    s = Server(seats, layers, n_head, n_kv, hd, page_size, n_pages, max_len, max_rows=int(lens.sum()))
+    d = n_head * hd
+    hist = [[[], []] for _ in range(seats)]          # k and v rows of the first layer, as given
+    g = torch.Generator(device=s.dev).manual_seed(2)
+
+    def note(counts):
+        at = 0
+        for r, c in enumerate(counts):
+            for i in (0, 1):
+                hist[r][i].append(s.first[i][at:at + c].clone())
+            at += c
+
+    def prompts(counts):
+        s.new.copy_(torch.as_tensor(np.asarray(counts, np.int32)))
+        s.forward(s.prompt_step, torch.randn((s.prompt_step.n_tokens, d), generator=g, device=s.dev).half())
+        note(counts)
+
+    prompts(lens)
+    s.new.fill_(1)
+    x = torch.zeros((seats, d), dtype=torch.float16, device=s.dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                    # the first decode step, which also warms the libraries up
+        x.copy_(torch.randn(x.shape, generator=g, device=s.dev))
+        s.forward(s.token_step, x)
+        note([1] * seats)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        s.forward(s.token_step, x)
+    graph_first = s.first
+    t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t0.record()
+    for _ in range(tokens):
+        x.copy_(torch.randn(x.shape, generator=g, device=s.dev))
+        graph.replay()
+        s.first = graph_first
+        note([1] * seats)
+    t1.record()
+    torch.cuda.synchronize()
+    s.check()
+
+    # every second session leaves; new prompts sit down in their seats while the others decode one token
+    gone = list(range(0, seats, 2))
+    before = int(s.n_free.item())
+    s.leave(gone)
+    freed = int(s.n_free.item()) - before
+    for r in gone:
+        hist[r] = [[], []]
+    prompts([max(1, int(n) // 2) if r in gone else 1 for r, n in enumerate(lens)])
+    s.check()
+
+    # the last step's attention of the first layer, over the rows as they were given
+    q, a = s.first[2].double().cpu().numpy(), s.first[3].double().cpu().numpy()
+    at, off, norm = 0, 0.0, 0.0
+    for r in range(seats):
+        n = sum(len(t) for t in hist[r][0])
+        assert n == int(s.held[r].item())
+        k, v = rotated(torch.cat(hist[r][0]), np.arange(n)), torch.cat(hist[r][1]).double().cpu().numpy()
+        c = len(hist[r][0][-1])
+        for h in range(n_head):
+            w = q[at:at + c, h] @ k[:, h // (n_head // n_kv)].T / np.sqrt(hd)
+            w = np.where(np.arange(n)[None] <= np.arange(n - c, n)[:, None], w, -np.inf)
+            w = np.exp(w - w.max(1, keepdims=True))
+            want = w @ v[:, h // (n_head // n_kv)] / w.sum(1, keepdims=True)
+            off, norm = off + ((a[at:at + c, h] - want) ** 2).sum(), norm + (want ** 2).sum()
+        at += c
+    return dict(ms_per_token_step=t0.elapsed_time(t1) / tokens, freed=freed, rows=at, rel_err=float(np.sqrt(off / norm)))
+
+
+if __name__ == "__main__":
+    p = argparse.ArgumentParser()
+    for name, value in (("seats", 8), ("prompt", 700), ("tokens", 64), ("layers", 4)):
+        p.add_argument("--" + name, type=int, default=value)
+    r = run(**vars(p.parse_args()))
+    print(f"{r['ms_per_token_step']:.3f} ms per decode step, {r['freed']} pages returned and taken again, "
+          f"attention over 8-bit rows against the rows as given: {r['rel_err']:.4f} of its norm")

@@ -64,6 +64,13 @@ cudaError_t launch_paged_append(const sv_paged& kv, const sv_paged_step& s, cons
                                 const sv_paged_rows& r, cudaStream_t st);
 cudaError_t launch_paged_read(const sv_paged& kv, const int32_t* slots, int n, void* k_out, void* v_out, int out_type,
                               cudaStream_t st);
+#ifdef __CUDACC__
+// log2 of a value scale, as both attention kernels put it into the exponent.  The append's smallest scale is above 2^-107;
+// codes of a page of zeros (scale 0) add nothing whatever stands here, and 2^-64 keeps their part of the row sum,
+// p' / vs, far from overflow.
+__device__ __forceinline__ float log2_scale(float vs) { return vs > 0.0f ? fmaxf(__log2f(vs), -107.0f) : -64.0f; }
+#endif
+
 struct PagedAttn {
     sv_paged kv;
     const int32_t* table;

@@ -22,7 +22,8 @@
 // The running maximum is lazy: a row's reference m_r moves only when a score passes it by 2^8, found by
 // a vote, so a tile normally needs no shuffle and no rescaling; p <= 2^8 is far inside f16.  P enters the second product
 // as two f16 parts (22 bits: with one, few rows' outputs were up to 1.6 times as far off as their own rounding); sums
-// stay f32.  P also carries vs / v_ref, where v_ref trails the largest vs seen by at most 4.
+// stay f32.  The value scale rides in the exponent: p' = vs p = exp2(s + log2 vs - m), m_r being the largest of s + log2 vs
+// so that f16's range serves the terms of the output whatever the scales; the row sum takes p' / vs.
 // The warps of a CTA meet pairwise in shared memory.  Segments of one request and head meet in the work space; the
 // last to arrive (a ticket) adds them in order, so results do not depend on which one that is.
 //
@@ -48,7 +49,7 @@ struct DecCfg {
     static constexpr int PITCH = HD + 4;                      // floats per row of a partial output
     static constexpr int BUFS = HD == 256 ? 1 : 2;            // warps whose partial outputs fit at once
     static constexpr int OFF_PART = STAGES * STAGE;           // float [BUFS][8 NT][PITCH]
-    static constexpr int OFF_SC = OFF_PART + BUFS * 8 * NT * PITCH * 4;   // float2 [STAGES][4]: each group's K and V scale
+    static constexpr int OFF_SC = OFF_PART + BUFS * 8 * NT * PITCH * 4;   // float2 [STAGES][4]: each group's K scale, log2 of its V scale
     static constexpr int OFF_OK = OFF_SC + STAGES * 32;       // int [STAGES][4]: the group's page exists
     static constexpr int OFF_BAR = OFF_OK + STAGES * 16;
     static constexpr int OFF_ML = OFF_BAR + STAGES * 16;      // float2 [kWarps][16]: maximum and sum, then int: last
@@ -195,7 +196,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 const float2 x = make_float2(__shfl_sync(0xffffffffu, b0.s.x, src), __shfl_sync(0xffffffffu, b0.s.y, src));
                 const int grp = 4 * (s.j0 + i) + (lane & 3);
                 if (lane < 4) {
-                    sc[st * 4 + lane] = make_float2(x.x * a.scale_log2, x.y);
+                    sc[st * 4 + lane] = make_float2(x.x * a.scale_log2, log2_scale(x.y));
                     okp[st * 4 + lane] = v;
                     if (!v && grp * 16 < s.rq.w && a.err) atomicOr(a.err, SV_DEVERR_PAGES);
                 }
@@ -231,7 +232,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     const int gq = lane >> 2, tq = lane & 3;
     const int k0 = gq & 1 ? gq ^ 4 : gq;                       // key of MMA index gq
     const int c0 = 2 * tq, c1 = (2 * tq + 1) ^ 4;              // keys of MMA indexes 2 tq, 2 tq + 1
-    int tile = 0;
+    int st = 0;
+    uint32_t ph = 0;
+    bool alive = true;
     for (int sg = g0; sg < g1; sg++) {
         const Seg sgm = seg_of(a, sg, sg == g0 ? cta : -1);
         const int4 rq = sgm.rq;
@@ -277,14 +280,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             for (int r = 0; r < NT; r++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[m][r][e] = 0.0f;
-        float mref[NT][2], l[NT][2], vref = 0.0f, vinv = 0.0f;
+        float mref[NT][2], l[NT][2];
 #pragma unroll
         for (int r = 0; r < NT; r++) mref[r][0] = mref[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
 
-        for (int i = 0; i < n; i++, tile++) {
-            const int st = tile % C::STAGES;
-            const bool got = mbar_wait(&full[st], (tile / C::STAGES) & 1, a.err);
-            if (!__all_sync(0xffffffffu, got)) return;             // the error bit is set; nothing can be trusted
+        for (int i = 0; i < n && alive; i++) {
+            alive = __all_sync(0xffffffffu, mbar_wait(&full[st], ph, a.err));
+            if (!alive) break;                                     // the error bit is set; the warps still meet below
             const int kb = (sgm.j0 + i) * kDecTile + 16 * warp;    // first key of this warp's group
             const float2 s2 = sc[st * 4 + warp];
             const bool there = okp[st * 4 + warp] != 0;
@@ -316,7 +318,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 #pragma unroll
                 for (int r = 0; r < NT; r++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[r][e] *= s2.x;
+                    for (int e = 0; e < 4; e++) s[r][e] = fmaf(s[r][e], s2.x, s2.y);
                 if (kb < lo_all || kb + 16 > hi_all) {
 #pragma unroll
                     for (int r = 0; r < NT; r++)
@@ -331,13 +333,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 for (int r = 0; r < NT; r++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) over |= s[r][e] > mref[r][e & 1] + kLazyLog2;
-                if (__any_sync(0xffffffffu, over || s2.y > 4.0f * vref)) {
-                    float vf = 1.0f;
-                    if (s2.y > vref) {
-                        vf = vref / s2.y;
-                        vref = s2.y;
-                        vinv = 1.0f / vref;
-                    }
+                if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                     for (int r = 0; r < NT; r++) {
                         float f[2];
@@ -347,10 +343,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 #pragma unroll
                             for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
                             const float mn = fmaxf(mref[r][e], mx);
-                            const float g = mn == -INFINITY ? 1.0f : fast_exp2(mref[r][e] - mn);
-                            l[r][e] *= g;
+                            f[e] = mn == -INFINITY ? 1.0f : fast_exp2(mref[r][e] - mn);
+                            l[r][e] *= f[e];
                             mref[r][e] = mn;
-                            f[e] = g * vf;
                         }
 #pragma unroll
                         for (int m = 0; m < HD / 16; m++)
@@ -358,7 +353,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                             for (int e = 0; e < 4; e++) o[m][r][e] *= f[e & 1];
                     }
                 }
-                const float pv = s2.y * vinv;
+                const float vinv = fast_exp2(-s2.y);
                 uint32_t pb[NT][2], pl[NT][2];                 // P as f16, and what that leaves of it
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
@@ -368,11 +363,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                         const float m = mref[r][e & 1];
                         p[e] = fast_exp2(s[r][e] - (m == -INFINITY ? 0.0f : m));
                     }
-                    l[r][0] += p[0] + p[2];
-                    l[r][1] += p[1] + p[3];
+                    l[r][0] = fmaf(p[0] + p[2], vinv, l[r][0]);
+                    l[r][1] = fmaf(p[1] + p[3], vinv, l[r][1]);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const float x = p[2 * e] * pv, y = p[2 * e + 1] * pv;
+                        const float x = p[2 * e], y = p[2 * e + 1];
                         const __half2 hp = __floats2half2_rn(x, y);
                         const float2 back = __half22float2(hp);
                         pb[r][e] = movm_t(*reinterpret_cast<const uint32_t*>(&hp));
@@ -415,6 +410,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
+            if (++st == C::STAGES) st = 0, ph ^= 1;
         }
         // ---- one partial of the CTA: the warps' maxima and sums, then outputs added (3, 2 into 1, 0, then 1 into 0; one
         // after the other with one buffer)
@@ -441,7 +437,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 float M = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w * 16 + 8 * r + 2 * tq + e].x);
-                const float f = mref[r][e] == -INFINITY ? 0.0f : vref * fast_exp2(mref[r][e] - M);
+                const float f = mref[r][e] == -INFINITY ? 0.0f : fast_exp2(mref[r][e] - M);
 #pragma unroll
                 for (int m = 0; m < HD / 16; m++) {
                     o[m][r][e] *= f;

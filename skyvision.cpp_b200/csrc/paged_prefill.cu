@@ -4,27 +4,35 @@
 //   s_rj = scale log2(e) ks[page(j)] (q_r . c_j),   p_rj = exp2(s_rj - m_r),
 //   o_r  = sum_j p_rj vs[page(j)] c'_j / sum_j p_rj
 // The scales belong to a page and head, so both products run on the codes alone, which are exact in f16: one MMA
-// part per tile where a block-scaled row format needs two.  ks is applied to finished scores, vs / v_ref to the
-// weights before they are rounded to f16 (see kTwoPartRows); sums stay f32.
+// part per tile where a block-scaled row format needs two.  ks is applied to finished scores; vs rides in the
+// exponent, p' = exp2(x + log2 vs - m_r), so that it costs nothing per weight and f16's range serves the terms of
+// the output however far apart the value scales are; the row sum takes each group's sum of p' times 1 / vs.  Sums
+// stay f32.
 //
 // Work item (from the plan): NQT tiles of 128 rows of one request and kv head (rows = tokens x the G query
 // heads, packed, so any G fills them) x a piece of the keys they see.  Roles:
 //   softmax warps   4 per row tile, one row per thread: S from TMEM, scales, causal / window mask, P as f16 back
 //                   over the S columns, 64 keys at a time so that O += P V starts on the first half.  No maximum
-//                   is taken as a rule: the weights are formed against the m_r at hand, and only where a row's sum
-//                   over the 64 keys passes 2^10 (far inside f16) or a row has no m_r yet is the maximum found, O in
-//                   TMEM and the sum rescaled, and the half formed again.
-//                   The V scales ride in the exponent: p' = exp2(x + log2 vs - v_ref), and the row sum takes each
-//                   group's share times 2^(v_ref - log2 vs), so they cost nothing per weight.
-//   converter warps read code tiles straight from the pages, turn bytes into f16 by permutes (0x64uu = 1024 + u;
-//                   minus 1152 is exact) and write them 128-byte swizzled into a ring of K and V tiles; the
-//                   loads of the next tile are issued as each piece of this one is stored.
+//                   is taken as a rule: the weights are formed against the m_r at hand, and only where a row's p'
+//                   over the 64 keys add up to more than 2^10 (far inside f16) or a row has no m_r yet is the
+//                   maximum of x + log2 vs found, O in TMEM and the sum rescaled, and the half formed again.
+//   TMA warp        looks up the pages and streams 64 keys of codes at a time (boxes of 16 keys, the smallest page)
+//                   into a staging ring.
+//   converter warps bytes -> f16 by permutes (0x64uu = 1024 + u; minus 1152 is exact), written 128-byte swizzled into
+//                   a ring of K and V tiles.  (Reading codes from global memory themselves, they stalled on it: 8192
+//                   rows 1.90 ms against 1.77 with the staging ring.)
 //   MMA warp        S = Q K^T (both K-major), O += P V (P from TMEM, V MN-major).
-// With two row tiles (HD 64, 128; 128 keys) each has one S buffer and they alternate on the tensor core; with
-// one (HD 256; 64 keys) S is double-buffered.
+// Two row tiles (HD 64, 128; tiles of 128 keys) have one S buffer each and alternate on the tensor core; one (HD
+// 256; 64 keys) has two.  64-key tiles with two S buffers at HD 128 were slower (twice the waits a key), as were two
+// threads per row (the row's sums meet through shuffles) and an MMA warp per row tile.
 // Pieces of an item's rows meet in the work space; the last to arrive adds them in order.
 //
-// Bound: tensor pipe and exponentials (4 NH HD flops and NH exponentials per visible pair).
+// Bound: 4 NH HD flops a visible pair on the tensor cores, 6 NH HD with P in two parts.
+// Measured (32 heads of 128 over 8): an 8192-token prompt beside 31 decoding sessions 1.75 ms, 980 TFLOP/s, 0.60 of a
+// large f16 GEMM's rate; the tensor pipe waits for the weights of the half that follows (64 exponentials a row
+// take as long as the MMAs of that half).  384 rows behind 4480 keys, two parts: 51 us, 790 TFLOP/s counting both; of
+// those 16 us are the start (query rows 5, first codes and S 5) and the merge of four pieces.  512 rows of 16 x 256
+// behind a window of 1024: 85 us.
 #include "common.cuh"
 #include "paged.hpp"
 #include "umma.cuh"
@@ -39,8 +47,6 @@ constexpr float kSumLimit = 1024.0f;      // a row's sum over 64 keys against it
 // scatters (up to 1.6 times seen in steps of 160 to 8192 rows, 1.47 in larger ones).  The second part costs 13 to 35 % of
 // the time (512 rows x 16 heads of 256: 74 -> 84 us; 8192 x 32 of 128: 1.77 -> 2.39 ms).
 constexpr int kTwoPartRows = 8192;
-constexpr float kVRefSlack = 2.0f;        // log2 vs may pass v_ref by this much before O is rescaled
-constexpr float kVFloor = -40.0f;         // log2 of the smallest vs / v_ref told apart (pages of zeros have vs = 0)
 
 template <int HD>
 struct PreCfgP {
@@ -197,7 +203,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
         const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, hi = min(pos + 1, rq.w);
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(qtl * C::QCOLS);
         // Scales of 32 groups at a time in this warp's own table: x = ks scale log2(e) (a page of zeros has zero
-        // scores at any x > 0; a group without a page has x < 0), y = log2 vs - v_ref, z = 2^-y.
+        // scores at any x > 0; a group without a page has x < 0), y = log2 vs, z = 2^-y.
         float4* tab = reinterpret_cast<float4*>(smem + C::OFF_SC) + warp * 32;
         constexpr int TPB = 32 / C::GROUPS;                 // tiles per batch of 32 groups
         auto scale_of = [&](int g, int p) {
@@ -240,24 +246,15 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
         }
-        float m = -INFINITY, l = 0.0f, vref = -INFINITY;
+        float m = -INFINITY, l = 0.0f;
         unsigned holes = 0;                                 // groups of the batch without a page
         bool ok = true;
         const int n_mine = tile_live ? n : 0;
         for (int i = 0; i < n_mine && ok; i++) {
             const int at = (i % TPB) * C::GROUPS;
-            float vmove = 1.0f;                             // factor on O when v_ref moves
             if (at == 0) {
                 const int g = (j0 + i) * C::GROUPS + lane;
-                const float lv = next.y > 0.0f ? __log2f(next.y) : -INFINITY;
-                float vm = lv;
-#pragma unroll
-                for (int w = 16; w > 0; w >>= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, w));
-                if (vm > vref + kVRefSlack) {
-                    if (vref > -INFINITY) vmove = fast_exp2(vref - vm);   // (zeros so far: O is 0)
-                    vref = vm;
-                }
-                const float y = fmaxf(lv - (vref > -INFINITY ? vref : 0.0f), kVFloor);
+                const float y = log2_scale(next.y);
                 __syncwarp();
                 tab[lane] = make_float4(next.x, y, fast_exp2(-y), 0.0f);
                 holes = __ballot_sync(0xffffffffu, next.x < 0.0f);
@@ -276,7 +273,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
             constexpr int CH = C::BN / 32;
             float s[2][32];
             uint32_t pk[32], pl[TWO ? 32 : 1];              // P as f16, and what that leaves of it
-            float sum = 0.0f;
+            float sum = 0.0f, top = 0.0f;                   // of p' / vs, and of p'
             auto mask = [&](float* x, int c) {              // this row's visible keys of 32
                 const int a0 = lo - kb - 32 * c, a1 = hi - kb - 32 * c;
                 const unsigned hole = holes >> (at + 2 * c);
@@ -306,7 +303,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                             w[8 * g + k / 2] = pack_h2(p.x, p.y);
                         }
                     }
-                    sum = fmaf(s2.x + s2.y, t.z, sum);
+                    const float g2 = s2.x + s2.y;
+                    top += g2;
+                    sum = fmaf(g2, t.z, sum);
                 }
             };
             tmem_ld32(sbuf, s[0]);
@@ -318,7 +317,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                 if (edge) mask(s[c & 1], c);
                 weights(s[c & 1], c, pk + 16 * (c & 1), pl + (TWO ? 16 * (c & 1) : 0));
                 if (c & 1) {
-                    if (__any_sync(0xffffffffu, !(sum <= kSumLimit) || m == -INFINITY) || (hf == 0 && vmove != 1.0f)) {
+                    if (__any_sync(0xffffffffu, !(top <= kSumLimit) || m == -INFINITY)) {
                         // the rows' maxima over this half, O and the sums to match, and the half once more
                         float t[32], mn = m;
 #pragma unroll 1
@@ -331,13 +330,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                                 float x = t[16 * g];
 #pragma unroll
                                 for (int j = 1; j < 16; j++) x = fmaxf(x, t[16 * g + j]);
-                                mn = fmaxf(mn, x * fabsf(tab[at + 2 * k + g].x));
+                                const float4 e = tab[at + 2 * k + g];
+                                mn = fmaxf(mn, fmaf(x, fabsf(e.x), e.y));
                             }
                         }
-                        float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+                        const float f = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
                         m = mn;
                         l *= f;
-                        if (hf == 0) f *= vmove;
                         if (i > 0 || hf > 0) {              // O must not be changing: the products issued so far are done
                             const bool done = hf > 0 ? warp_wait(&o_half[qtl], i & 1, a.err, abort_flag)
                                                      : warp_wait(&o_done[2 * qtl + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err, abort_flag);
@@ -362,7 +361,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
                         }
                     }
                     l += sum;
-                    sum = 0.0f;
+                    sum = top = 0.0f;
                     tmem_st32(sbuf + 64 * hf, reinterpret_cast<const float*>(pk));     // over the half's own columns
                     if constexpr (TWO) tmem_st32(sbuf + 64 * hf + 32, reinterpret_cast<const float*>(pl));
                 }
@@ -380,14 +379,13 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
             ok = false;
         tc_fence_after();
         const bool have = n_mine > 0 && ok;
-        const float vscale = vref > -INFINITY ? fast_exp2(vref) : 1.0f;     // O is in units of it
-        auto load_o = [&](int cc, float* o, float f) {
+        auto load_o = [&](int cc, float* o) {
             if (have) {
                 tmem_ld32(lane_addr + C::SCOLS + cc, o);
                 tmem_wait_ld();
             }
 #pragma unroll
-            for (int k = 0; k < 32; k++) o[k] = have ? o[k] * f : 0.0f;
+            for (int k = 0; k < 32; k++) o[k] = have ? o[k] : 0.0f;
         };
         const size_t orow = ((size_t)(rq.x + tok) * a.n_head + hd) * HD;
         auto store = [&](int cc, const float* o, float f) {
@@ -409,7 +407,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
 #pragma unroll 1
             for (int cc = 0; cc < HD; cc += 32) {
                 float o[32];
-                load_o(cc, o, vscale);
+                load_o(cc, o);
                 store(cc, o, inv);
             }
         } else {
@@ -421,7 +419,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
 #pragma unroll 1
             for (int cc = 0; cc < HD; cc += 32) {
                 float o[32];
-                load_o(cc, o, vscale);
+                load_o(cc, o);
                 if (tile_live) {
 #pragma unroll
                     for (int k = 0; k < 8; k++)
@@ -552,8 +550,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
             for (int k = max(0, e - C::NR); k < e; k++) mbar_wait(&raw_full[k % C::NR], (k / C::NR) & 1, a.err);
         } else if (warp == C::SM_WARPS + C::CV_WARPS && nu > 0) {
             // ======================== MMA issuer: the whole warp runs the loop and one elected lane issues, so that the
-            // descriptors are uniform values (held per thread they had to be moved to uniform registers before each MMA:
-            // 109 cycles between MMAs of 64)
+            // descriptors are the same on all lanes (one lane running the loop alone: 8192 rows 1.99 ms against 1.90)
             const uint32_t idesc_s = umma_idesc(128, C::BN, 0, 0), idesc_o = umma_idesc(128, HD, 0, 1);
             constexpr uint32_t hi = desc_hi_sw128(1024);
             const uint32_t q_lo = desc_lo(smem_u32(smem), 16);

@@ -567,3 +567,123 @@ def test_refusals():
                 dict(n_dims=64, freq_scale=0.0), dict(n_dims=64, ext_factor=1.0), dict(n_dims=64, freq_factors=[1.0])):
         with pytest.raises(sv.SvError):
             sv.Rope(**bad)
+
+
+# ------------------------------------------------------------------ large steps, long pools, rows that are no numbers
+@pytest.mark.parametrize("past,new,hd,ps,nh,nkv", [([0], [1100], 64, 16, 8, 2), ([700, 0, 33], [600, 450, 1], 128, 32, 8, 2),
+                                                   ([100], [1030], 256, 64, 8, 1), ([40, 5], [129, 900], 128, 128, 9, 3),
+                                                   ([0] * 9, [250] * 9, 64, 32, 4, 4)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_attn_large_steps(past, new, hd, ps, nh, nkv, window):
+    """More query rows in the step than the small-step kernels take: the weights go as one f16 each."""
+    b = Batch(34, past, new, hd=hd, ps=ps, n_head=nh, n_kv=nkv).plan()
+    assert b.T * nh > 8192
+    _attn(b, b.fill(), window=window)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attn_large_steps_scales_far_apart(hd):
+    b = Batch(35, [300, 20], [700, 400], hd=hd, ps=16, n_head=8, n_kv=2).plan()
+    _attn(b, b.fill(k_spread=1.0, v_spread=2.0), out=torch.float32)
+
+
+@pytest.mark.parametrize("past,new", [([3000], [1]), ([300, 20], [3, 5]), ([700, 40], [150, 90]), ([10], [1100])])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attn_rows_that_are_no_numbers_stay_alone(past, new, hd):
+    """A query row with NaN, infinities or values past f16's range changes no other row's bits."""
+    b = Batch(36, past, new, hd=hd, ps=16, n_head=8, n_kv=2).plan()
+    b.fill()
+    q = torch.from_numpy(b.rng.standard_normal((b.T, 8, hd))).to(DEV, torch.float32)
+    first = b.kv.attn(0, b.step, q, 0.1)
+    bad = q.clone()
+    rows = torch.zeros((b.T, 8), dtype=torch.bool, device=DEV)
+    for t in range(0, b.T, 37):
+        for h, x in ((1, float("nan")), (2, float("inf")), (6, 1e30)):
+            bad[t, h, 5] = x
+            rows[t, h] = True
+    out = b.kv.attn(0, b.step, bad, 0.1)
+    # (a row's reference may be taken earlier because of its neighbours, so the weights' rounding differs: twice the
+    # tolerance of one output)
+    big = max(float(b.kv.scales(0, 1).max()) * 127, 1e-30)
+    tol = 2 * (2.0 ** -10 * big + 2.0 ** -11 * first[~rows].double().abs())
+    assert ((out[~rows].double() - first[~rows].double()).abs() <= tol).all()
+    assert b.kv.error_flags() == 0
+
+
+@pytest.mark.parametrize("past,new", [([3000], [1]), ([500, 64], [2, 1]), ([600, 31], [200, 161]), ([100], [1100])])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window", [16, 0])
+def test_attn_rows_of_small_values_beside_large_ones(past, new, hd, window):
+    """Value scales 2^22 apart from page to page: a row whose window (or whose weights) holds small values alone is as
+    exact as any other, against the largest |weight x value| that it sees."""
+    b = Batch(38, past, new, hd=hd, ps=16, n_head=8, n_kv=2).plan()
+    k, v, ks, vs = b.fill()
+    _, kv_len, _, _, _, table, _ = b.want()
+    for r, n in enumerate(kv_len):
+        for j in range(-(-n // 16)):
+            p = int(table[r, j])
+            vs[p] *= 2.0 ** -22 if j % 2 else 1.0
+            if window == 0:                           # keys of the large values get no weight: 50 binary orders less
+                k[p] = -8 if j % 2 == 0 else 8
+                ks[p] = 0.05
+    for is_v, (c, s) in enumerate(((k, ks), (v, vs))):
+        b.kv.codes(0, is_v).copy_(torch.from_numpy(np.ascontiguousarray(c).astype(np.int8)))
+        b.kv.scales(0, is_v).copy_(torch.from_numpy(s.astype(np.float32)))
+    q = b.rng.standard_normal((b.T, 8, hd)) * 0.01
+    if window == 0:
+        q = np.abs(q) + 50 * np.log(2) / (2 * 0.4 * hd * 0.5)
+    q = torch.from_numpy(q).to(DEV, torch.float16)
+    got = _np(b.kv.attn(0, b.step, q, 0.5, window=window, out=torch.empty((b.T, 8, hd), dtype=torch.float32, device=DEV)))
+    qd = _np(q)
+    want = orc.attention(qd, k, v, ks, vs, table, b.past, b.new, kv_len, 0.5, window)
+    # the same with |v| and, per row, the largest weight x scale in place of the sum
+    t = 0
+    for r, c in enumerate(b.new):
+        for i in range(c):
+            p = b.past[r] + i
+            lo, hi = (max(0, p - window + 1) if window else 0), min(p + 1, kv_len[r])
+            pages = np.array([int(table[r, j // 16]) for j in range(lo, hi)])
+            at = np.arange(lo, hi) % 16
+            for h in (0, 7):
+                x = (k[pages, h // 4, at] * ks[pages, h // 4][:, None].astype(np.float64)) @ qd[t, h] * 0.5
+                w = np.exp(x - x.max())
+                each = w[:, None] * np.abs(v[pages, h // 4, at]) * vs[pages, h // 4][:, None].astype(np.float64) / w.sum()
+                tol = 2.0 ** -10 * each.sum(0) + 2.0 ** -20 * each.max()
+                assert np.all(np.abs(got[t, h] - want[t, h]) <= tol)
+            t += 1
+    assert b.kv.error_flags() == 0
+
+
+def test_pool_past_32_bit_offsets():
+    """The pages of a step lie beyond 2^31 bytes and 2^31 elements of the pool: the same bits as in a small pool."""
+    hd, nkv, nh, ps, past, new = 256, 8, 16, 128, [300, 70], [1, 200]
+    small = Batch(37, [0, 0], [p + n for p, n in zip(past, new)], hd=hd, ps=ps, n_head=nh, n_kv=nkv)
+    rows = torch.from_numpy(small.rng.standard_normal((sum(past) + sum(new), nh + 2 * nkv, hd))).to(DEV, torch.float16)
+    outs = []
+    for n_pages in (small.n_pages, 9000):
+        kv = sv.PagedKv(1, nkv, hd, ps, n_pages)
+        free = _i(np.arange(n_pages))               # the last are taken first
+        table, nf = _i(np.full((2, 4), -1)), _i([n_pages])
+        got, rope = [], sv.Rope(hd)
+        for had, add, x in (([0, 0], past, rows[:sum(past)]), (past, new, rows[sum(past):])):
+            step = sv.PagedStep(2, sum(add), max(add), ps, n_pages, nh, nkv, hd)
+            step.plan(_i(had), _i(add), table, free, nf)
+            nf = step.n_free.clone()
+            q = kv.rope_append(0, step, x[:, :nh], x[:, nh:nh + nkv], x[:, nh + nkv:], rope=rope)
+            got += [q, kv.attn(0, step, q, 0.07)]
+            k, v = kv.read(0, step.tok_slot)
+            got += [k, v]
+            assert step.error_flags() == 0 and kv.error_flags() == 0
+        if n_pages == 9000:
+            assert int(table[table >= 0].min()) * nkv * ps * hd > 2 ** 31
+        outs.append(got)
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
+def test_example_sessions():
+    """The example at a small size.  Codes carry values to s / sqrt(12) with s = max / 127 over a page and head (about 3.5
+    to 4 standard deviations): 0.9 % of a row, and again each time a page's scale grows; K's part moves the weights by as
+    much.  Together below 4 % of the output's norm."""
+    from examples.paged_sessions import run
+    r = run(seats=5, prompt=150, tokens=12, layers=2, n_head=8, n_kv=2, hd=64, page_size=16)
+    assert r["freed"] > 0 and r["rel_err"] < 0.04
