@@ -27,7 +27,10 @@
 // The warps of a CTA meet pairwise in shared memory.  Segments of one request and head meet in the work space; the
 // last to arrive (a ticket) adds them in order, so results do not depend on which one that is.
 //
-// Bound: HBM, 2 HD + 8 / page_size bytes per key and kv head.
+// Bound: HBM, 2 HD + 8 / page_size bytes per key and kv head.  Measured in a graph (8 kv heads of 128, 4 query heads
+// each): 64 requests of 512 to 32768 keys, 2.2 GB: 363 us, 6.1 TB/s, 0.93 of a copy's rate; one of 131072: 56 us, 4.8
+// TB/s (start, first tiles and the merge of 55 pieces are 15 us of it); one of 4481: 11 us, all of it latency.
+// Equal pieces against a request's own splits: 363 and 56 us against 547 and 77.
 #include "common.cuh"
 #include "paged.hpp"
 

@@ -9,6 +9,8 @@
 // new entry and the step's page record, so there are no atomics and the order is fixed.
 //
 // Bound: latency (a launch, two dependent loads, the scans); the step's arrays are a few hundred KB.
+// Measured in a graph: 4.2 us for eight decoding requests (128 threads a block: a scan's barriers span four warps), 13.7
+// for 1000 requests of up to 64 rows (512 threads; 64-bit scans of all sums took 26).
 #include "common.cuh"
 #include "paged.hpp"
 
@@ -62,7 +64,8 @@ __device__ __forceinline__ int find_last(const int* start, int n, int x) {
 
 // Piece length (in tiles) for units of cost(u) tiles each.  Up to `slots` units: the shortest that gives no more than
 // `slots` items, so all run at once.  Up to kMoreWaves times as many: pieces of a kMoreWaves-th of an even share, so that the last
-// wave is short.  More units than that: whole units.  At least min_tiles in any case.
+// wave is short (31 decoding requests beside a prompt of 8192: the last wave's idle SMs cost up to a unit's time, pieces a
+// merge).  More units than that: whole units.  At least min_tiles in any case.
 constexpr int kMoreWaves = 3;
 template <int kThreads, class Cost>
 __device__ int piece_of(int n_units, int slots, int min_tiles, Cost cost, long long* buf) {

@@ -28,11 +28,11 @@
 // Pieces of an item's rows meet in the work space; the last to arrive adds them in order.
 //
 // Bound: 4 NH HD flops a visible pair on the tensor cores, 6 NH HD with P in two parts.
-// Measured (32 heads of 128 over 8): an 8192-token prompt beside 31 decoding sessions 1.75 ms, 980 TFLOP/s, 0.60 of a
+// Measured (32 heads of 128 over 8): an 8192-token prompt part beside 31 decoding sessions 1.75 ms, 980 TFLOP/s, 0.60 of a
 // large f16 GEMM's rate; the tensor pipe waits for the weights of the half that follows (64 exponentials a row
-// take as long as the MMAs of that half).  384 rows behind 4480 keys, two parts: 51 us, 790 TFLOP/s counting both; of
+// take as long as the MMAs of that half).  384 tokens behind 4096 keys: 51 us, 530 TFLOP/s; of
 // those 16 us are the start (query rows 5, first codes and S 5) and the merge of four pieces.  512 rows of 16 x 256
-// behind a window of 1024: 85 us.
+// behind a window of 4096: 85 us.
 #include "common.cuh"
 #include "paged.hpp"
 #include "umma.cuh"
