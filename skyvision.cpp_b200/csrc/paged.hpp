@@ -33,6 +33,9 @@ constexpr int pre_rows(int hd) { return hd == 256 ? 128 : 256; }   // query rows
 constexpr int pre_tile(int hd) { return hd == 256 ? 64 : 128; }    // keys per prefill tile
 // a split shorter than this costs more in its start and merge than it saves
 constexpr int kDecMinTiles = 6;
+// where requests are so many that they share CTAs: an even share of the line, down to this (200 requests of one tile: 15.5 us,
+// 21.2 with six)
+constexpr int kDecShareTiles = 2;
 constexpr int kPreMinTiles = 4;
 
 enum : int { PH_PAGES = 0, PH_PRE = 1 };

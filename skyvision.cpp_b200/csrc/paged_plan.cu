@@ -9,7 +9,7 @@
 // new entry and the step's page record, so there are no atomics and the order is fixed.
 //
 // Bound: latency (a launch, two dependent loads, the scans); the step's arrays are a few hundred KB.
-// Measured in a graph: 4.2 us for eight decoding requests (128 threads a block: a scan's barriers span four warps), 13.7
+// Measured in a graph: 4.5 us for eight decoding requests (128 threads a block: a scan's barriers span four warps), 13.7
 // for 1000 requests of up to 64 rows (512 threads; 64-bit scans of all sums took 26).
 #include "common.cuh"
 #include "paged.hpp"
@@ -220,7 +220,9 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
         }
         for (int i = threadIdx.x; i < a.l.n_ticks; i += kThreads) reinterpret_cast<int*>(work + a.l.tick)[i] = 0;
         // ---- decode: the key tiles of all requests of few rows form one line, cut into equal pieces, a CTA each; a
-        // piece's part of a request is a segment
+        // piece's part of a request is a segment.  Where the CTAs suffice each request starts a piece of its own (the line has
+        // gaps): a segment costs about 2 us whatever its length, and those of one CTA follow one another (13 requests of
+        // one tile and eight kv heads: 18.7 us in three CTAs a head, 5.2 apart).
         int4* dec = reinterpret_cast<int4*>(work + a.l.dec);
         int* cta = reinterpret_cast<int*>(work + a.l.cta);
         int4* head_seg = reinterpret_cast<int4*>(work + a.l.head_seg);
@@ -238,17 +240,33 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
                 for (int r = threadIdx.x; r < n; r += kThreads) sum += dec_cost(r);
                 block_scan<kThreads, int>(sum, &line, reinterpret_cast<int*>(buf));
             }
-            int t0 = 0, base = 0, piece = 0;
+            int t0 = 0, base = 0, piece = 0, ctas = 0;
             for (int u0 = 0; u0 < n; u0 += kThreads) {
                 const int r = u0 + threadIdx.x;
                 const int c = r < n ? dec_cost(r) : 0;
-                int all, segs;
-                const int t = t0 + block_scan<kThreads, int>(c, &all, reinterpret_cast<int*>(buf));
+                int all, segs, ns = 0, at = 0;
+                int t = t0 + block_scan<kThreads, int>(c, &all, reinterpret_cast<int*>(buf));
                 t0 += all;
                 if (one) line = all;
-                if (u0 == 0) piece = max((line + a.l.dec_slots - 1) / a.l.dec_slots, kDecMinTiles);
-                const int p0 = t / piece, ns = c > 0 ? (t + c - 1) / piece - p0 + 1 : 0;
-                const int at = base + block_scan<kThreads, int>(ns, &segs, reinterpret_cast<int*>(buf));
+                bool apart = false;
+                if (u0 == 0) {
+                    const int share = (line + a.l.dec_slots - 1) / a.l.dec_slots;
+                    piece = max(share, kDecMinTiles);
+                    if (one) {
+                        ns = (c + piece - 1) / piece;
+                        at = block_scan<kThreads, int>(ns, &segs, reinterpret_cast<int*>(buf));
+                        apart = segs <= a.l.dec_slots;
+                    }
+                    if (!apart) piece = max(share, kDecShareTiles);
+                    ctas = apart ? segs : (line + piece - 1) / piece;
+                }
+                if (apart) {
+                    t = at * piece;
+                } else {
+                    ns = c > 0 ? (t + c - 1) / piece - t / piece + 1 : 0;
+                    at = base + block_scan<kThreads, int>(ns, &segs, reinterpret_cast<int*>(buf));
+                }
+                const int p0 = t / piece;
                 base += segs;
                 const int4 q = ns > 0 ? req_of(r) : make_int4(0, 0, 0, 0);
                 for (int i = 0; i < ns; i++) {
@@ -263,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const __grid_const
                     }
                 }
             }
-            for (int i = (line + piece - 1) / piece + threadIdx.x; i <= a.l.dec_slots; i += kThreads) cta[i] = base;
+            for (int i = ctas + threadIdx.x; i <= a.l.dec_slots; i += kThreads) cta[i] = base;
         }
         // ---- prefill items: query tiles of the other requests, last ones (most keys) first
         int4* pre = reinterpret_cast<int4*>(work + a.l.pre);

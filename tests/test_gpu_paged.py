@@ -654,6 +654,17 @@ def test_attn_rows_of_small_values_beside_large_ones(past, new, hd, window):
     assert b.kv.error_flags() == 0
 
 
+@pytest.mark.parametrize("n", [9, 36, 37, 38, 54, 55, 56, 57, 130, 200])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attn_many_short_requests(n, hd):
+    """About as many requests, and pieces of requests, as thread blocks run at once, and more of either."""
+    rng = np.random.default_rng(n)
+    for hi in (30, 500):
+        past, new = rng.integers(0, hi, n).tolist(), rng.integers(0, 3, n).tolist()
+        b = Batch(39, past, new, hd=hd, ps=32, n_head=8, n_kv=8).plan()
+        _attn(b, b.fill())
+
+
 def test_pool_past_32_bit_offsets():
     """The pages of a step lie beyond 2^31 bytes and 2^31 elements of the pool: the same bits as in a small pool."""
     hd, nkv, nh, ps, past, new = 256, 8, 16, 128, [300, 70], [1, 200]
