@@ -42,6 +42,7 @@ enum : int { PH_PAGES = 0, PH_PRE = 1 };
 
 struct StepLayout {
     int page_cap = 0, dec_cap = 0, pre_cap = 0;     // most entries of each list
+    int pre_units = 0;                              // most prefill units
     int few = kDecRows;                             // rows of a decode unit, at most
     int dec_slots = 1, pre_slots = 1;               // CTAs that run at once, per kv head
     size_t head = 0, req = 0, page = 0, dec = 0, cta = 0, head_seg = 0, pre = 0, tick = 0, dec_part = 0, dec_ml = 0, pre_part = 0, pre_ml = 0;
@@ -84,6 +85,7 @@ struct PagedAttn {
     size_t q_nb;
     float scale_log2;
     int window;
+    int join;                // prefill: the pieces are added by a kernel of their own
     void* out;
     int out_type;
     uint8_t* work;

@@ -377,7 +377,8 @@ bool step_layout(const sv_paged_step& s, StepLayout* l) {
     const int rows = pre_rows(s.head_dim);
     if ((int64_t)max_new * G > l->few) {
         const int64_t least = l->few / G + 1;    // fewest tokens of a prefill request
-        l->pre_cap = (int)(T * G / rows + (act < T / least ? act : T / least) + kMoreWaves * l->pre_slots);
+        l->pre_units = (int)(T * G / rows + (act < T / least ? act : T / least));
+        l->pre_cap = l->pre_units + kMoreWaves * l->pre_slots;
     }
     size_t at = 0;
     auto take = [&](size_t bytes) {

@@ -25,7 +25,8 @@
 // Two row tiles (HD 64, 128; tiles of 128 keys) have one S buffer each and alternate on the tensor core; one (HD
 // 256; 64 keys) has two.  64-key tiles with two S buffers at HD 128 were slower (twice the waits a key), as were two
 // threads per row (the row's sums meet through shuffles) and an MMA warp per row tile.
-// Pieces of an item's rows meet in the work space; the last to arrive adds them in order.
+// Pieces of a unit's rows meet in the work space and are added in order: by the last to arrive, behind the others' work, or, of
+// a step whose few units are cut into many pieces, by a second kernel over all SMs.
 //
 // Bound: 4 NH HD flops a visible pair on the tensor cores, 6 NH HD with P in two parts.
 // Measured (32 heads of 128 over 8): an 8192-token prompt part beside 31 decoding sessions 1.75 ms, 980 TFLOP/s, 0.60 of a
@@ -420,53 +421,55 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
             for (int cc = 0; cc < HD; cc += 32) {
                 float o[32];
                 load_o(cc, o);
-                if (tile_live) {
+                if (live) {
 #pragma unroll
                     for (int k = 0; k < 8; k++)
                         wo[(size_t)(cc / 4 + k) * C::ROWS + flat] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                 }
             }
-            if (tile_live) mls[unit * C::ROWS + flat] = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
-            __threadfence();
-            asm volatile("barrier.sync 2, %0;" ::"n"(C::SM_WARPS * 32) : "memory");
-            if (threadIdx.x == 0) {
-                int* ticket = reinterpret_cast<int*>(a.work + a.l.tick) + (size_t)a.l.dec_cap * NKV + first;
-                const int last = atomicAdd(ticket, 1) == ns - 1;
-                if (last) *ticket = 0;                     // ready for the next layer
-                *s_last = last;
-            }
-            asm volatile("barrier.sync 2, %0;" ::"n"(C::SM_WARPS * 32) : "memory");
-            if (*s_last && tile_live) {
+            if (live) mls[unit * C::ROWS + flat] = make_float2(have ? m : -INFINITY, have ? l : 0.0f);
+            if (!a.join) {                                 // the last to arrive adds them, in order
                 __threadfence();
-                const size_t so = (size_t)NKV * C::ROWS;
-                const float2* ml = mls + first * C::ROWS + flat;
-                float M = -INFINITY, L = 0.0f;
-                for (int sp = 0; sp < ns; sp++) M = fmaxf(M, __ldcg(ml + sp * so).x);
-                for (int sp = 0; sp < ns; sp++) {
-                    const float2 x = __ldcg(ml + sp * so);
-                    L += x.x == -INFINITY ? 0.0f : x.y * fast_exp2(x.x - M);
+                asm volatile("barrier.sync 2, %0;" ::"n"(C::SM_WARPS * 32) : "memory");
+                if (threadIdx.x == 0) {
+                    int* ticket = reinterpret_cast<int*>(a.work + a.l.tick) + (size_t)a.l.dec_cap * NKV + first;
+                    const int last = atomicAdd(ticket, 1) == ns - 1;
+                    if (last) *ticket = 0;                     // ready for the next layer
+                    *s_last = last;
                 }
-                const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-#pragma unroll 1
-                for (int cc = 0; cc < HD; cc += 32) {
-                    float o[32];
-#pragma unroll
-                    for (int k = 0; k < 32; k++) o[k] = 0.0f;
+                asm volatile("barrier.sync 2, %0;" ::"n"(C::SM_WARPS * 32) : "memory");
+                if (*s_last && live) {
+                    __threadfence();
+                    const size_t so = (size_t)NKV * C::ROWS;
+                    const float2* ml = mls + first * C::ROWS + flat;
+                    float M = -INFINITY, L = 0.0f;
+                    for (int sp = 0; sp < ns; sp++) M = fmaxf(M, __ldcg(ml + sp * so).x);
                     for (int sp = 0; sp < ns; sp++) {
-                        const float x = __ldcg(ml + sp * so).x, w = x == -INFINITY ? 0.0f : fast_exp2(x - M);
-                        const float4* p = part + (first + (size_t)sp * NKV) * C::ROWS * (HD / 4) + (size_t)(cc / 4) * C::ROWS + flat;
-                        float4 v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = __ldcg(p + (size_t)k * C::ROWS);
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            o[4 * k] = fmaf(w, v[k].x, o[4 * k]);
-                            o[4 * k + 1] = fmaf(w, v[k].y, o[4 * k + 1]);
-                            o[4 * k + 2] = fmaf(w, v[k].z, o[4 * k + 2]);
-                            o[4 * k + 3] = fmaf(w, v[k].w, o[4 * k + 3]);
-                        }
+                        const float2 x = __ldcg(ml + sp * so);
+                        L += x.x == -INFINITY ? 0.0f : x.y * fast_exp2(x.x - M);
                     }
-                    store(cc, o, inv);
+                    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll 1
+                    for (int cc = 0; cc < HD; cc += 32) {
+                        float o[32];
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] = 0.0f;
+                        for (int sp = 0; sp < ns; sp++) {
+                            const float x = __ldcg(ml + sp * so).x, w = x == -INFINITY ? 0.0f : fast_exp2(x - M);
+                            const float4* p = part + (first + (size_t)sp * NKV) * C::ROWS * (HD / 4) + (size_t)(cc / 4) * C::ROWS + flat;
+                            float4 v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) v[k] = __ldcg(p + (size_t)k * C::ROWS);
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                o[4 * k] = fmaf(w, v[k].x, o[4 * k]);
+                                o[4 * k + 1] = fmaf(w, v[k].y, o[4 * k + 1]);
+                                o[4 * k + 2] = fmaf(w, v[k].z, o[4 * k + 2]);
+                                o[4 * k + 3] = fmaf(w, v[k].w, o[4 * k + 3]);
+                            }
+                        }
+                        store(cc, o, inv);
+                    }
                 }
             }
         }
@@ -638,6 +641,81 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_const
     }
 }
 
+// Adds the pieces of the units that were cut: 32 rows and one kv head at a time, a row per lane, the columns over the warps.
+//   M = max m_p,  o = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p
+// Bound: L2, the pieces have just been written.  For units that may be cut into kJoinPieces or more, all at once: 16 tokens
+// over 8000 keys (16 pieces) 41 -> 31 us, 128 tokens of 16 x 256 over 1000 (5 pieces) 36 -> 28; with fewer the launch costs what it
+// saves (384 tokens over 4096 keys, three pieces: 51.4 against 52.6), and pieces of several waves are added behind others' work
+// for nothing (2048 tokens: 70 against 89).
+constexpr int kJoinPieces = 4;
+constexpr int kJoinWarps = 8;
+template <int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn a) {
+    constexpr int ROWS = pre_rows(HD), CHUNKS = ROWS / 32, K = HD / 4 / kJoinWarps;   // float4 columns per thread
+    constexpr int U = 16 / K < 8 ? 16 / K : 8;                                       // pieces whose loads are in flight
+    __shared__ float s_m[kJoinWarps][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, NKV = a.kv.n_kv_head;
+    pdl_wait();
+    if (threadIdx.x == 0) pdl_trigger();
+    const int n_items = reinterpret_cast<const int*>(a.work + a.l.head)[PH_PRE];
+    const int n_work = n_items * NKV * CHUNKS;
+    for (int w = blockIdx.x; w < n_work; w += gridDim.x) {
+        const int item = w / (NKV * CHUNKS), h = w / CHUNKS % NKV, r = w % CHUNKS * 32 + lane;
+        const int4 it = reinterpret_cast<const int4*>(a.work + a.l.pre)[item];
+        const int4 rq = reinterpret_cast<const int4*>(a.work + a.l.req)[it.x];
+        const int ns = it.w, row = it.y * ROWS + r, n_rows = rq.y * a.G;
+        if (it.z != 0 || ns == 1 || row - lane >= n_rows) continue;
+        const bool live = row < n_rows;
+        const size_t first = (size_t)item * NKV + h, so = (size_t)NKV * ROWS;
+        const float2* ml = reinterpret_cast<const float2*>(a.work + a.l.pre_ml) + first * ROWS + r;
+        float M = -INFINITY;
+        for (int s = warp; s < ns; s += kJoinWarps) M = fmaxf(M, live ? __ldcg(ml + s * so).x : -INFINITY);
+        __syncthreads();                                           // the unit before has been read
+        s_m[warp][lane] = M;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kJoinWarps; k++) M = fmaxf(M, s_m[k][lane]);
+        if (!live) continue;
+        const float4* part = reinterpret_cast<const float4*>(a.work + a.l.pre_part) + first * ROWS * (HD / 4) +
+                             (size_t)(warp * K) * ROWS + r;
+        float4 o[K];
+        float L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < ns; s0 += U) {
+            float2 x[U];
+            float4 y[U][K];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int s = min(s0 + u, ns - 1);
+                x[u] = __ldcg(ml + s * so);
+#pragma unroll
+                for (int k = 0; k < K; k++) y[u][k] = __ldcg(part + s * so * (HD / 4) + (size_t)k * ROWS);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float f = s0 + u >= ns || x[u].x == -INFINITY ? 0.0f : fast_exp2(x[u].x - M);
+                L = fmaf(f, x[u].y, L);
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    o[k].x = fmaf(f, y[u][k].x, o[k].x);
+                    o[k].y = fmaf(f, y[u][k].y, o[k].y);
+                    o[k].z = fmaf(f, y[u][k].z, o[k].z);
+                    o[k].w = fmaf(f, y[u][k].w, o[k].w);
+                }
+            }
+        }
+        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+        const size_t at = ((size_t)(rq.x + row / a.G) * a.n_head + h * a.G + row % a.G) * HD + warp * K * 4;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const float4 v = make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+            if (a.out_type == SV_TYPE_F32) reinterpret_cast<float4*>(static_cast<float*>(a.out) + at)[k] = v;
+            else reinterpret_cast<uint2*>(static_cast<__half*>(a.out) + at)[k] = make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
+        }
+    }
+}
+
 template <int HD, bool TWO>
 cudaError_t launch_parts(const PagedAttn& a, cudaStream_t st) {
     using C = PreCfgP<HD>;
@@ -654,8 +732,12 @@ cudaError_t launch_parts(const PagedAttn& a, cudaStream_t st) {
     if (!encode_tmap_2d(&tmk, a.kv.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz) ||
         !encode_tmap_2d(&tmv, a.kv.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, HD, rows, HD, C::COLS, 16, swz))
         return cudaErrorInvalidValue;
-    return launch_pdl(paged_prefill_kernel<HD, TWO>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)), dim3(C::THREADS), (size_t)smem, st,
-                      tmk, tmv, a);
+    const cudaError_t launched = launch_pdl(paged_prefill_kernel<HD, TWO>, dim3((unsigned)(a.l.pre_cap * a.kv.n_kv_head)),
+                                            dim3(C::THREADS), (size_t)smem, st, tmk, tmv, a);
+    if (launched != cudaSuccess) return launched;
+    if (!a.join) return cudaSuccess;
+    const int64_t most = (int64_t)a.l.pre_cap * a.kv.n_kv_head * (C::ROWS / 32), full = 4 * (int64_t)device_sm_count();
+    return launch_pdl(paged_join_kernel<HD>, dim3((unsigned)(most < full ? most : full)), dim3(kJoinWarps * 32), 0, st, a);
 }
 
 template <int HD>
@@ -665,8 +747,10 @@ cudaError_t launch_hd(const PagedAttn& a, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_paged_prefill(const PagedAttn& a, cudaStream_t st) {
+cudaError_t launch_paged_prefill(const PagedAttn& args, cudaStream_t st) {
+    PagedAttn a = args;
     if (a.l.pre_cap == 0) return cudaSuccess;
+    a.join = (int64_t)kJoinPieces * a.l.pre_units <= a.l.pre_slots;
     switch (a.kv.head_dim) {
         case 64: return launch_hd<64>(a, st);
         case 128: return launch_hd<128>(a, st);
