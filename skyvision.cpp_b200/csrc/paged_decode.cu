@@ -28,7 +28,8 @@
 // last to arrive (a ticket) adds them in order, so results do not depend on which one that is.
 //
 // Bound: HBM, 2 HD + 8 / page_size bytes per key and kv head.  Measured in a graph (8 kv heads of 128, 4 query heads
-// each): 64 requests of 512 to 32768 keys, 2.2 GB: 363 us, 6.1 TB/s, 0.93 of a copy's rate; one of 131072: 56 us, 4.8
+// each): 64 requests of 512 to 32768 keys, 2.2 GB: 363 us, 6.1 TB/s, 0.93 of a copy's rate (at 1965 MHz; 415 to 431 where the
+// power cap holds the SM clock at 1575 to 1800: then it is the instructions per key that count); one of 131072: 56 us, 4.8
 // TB/s (start, first tiles and the merge of 55 pieces are 15 us of it); one of 4481: 11 us, all of it latency.
 // Equal pieces against a request's own splits: 363 and 56 us against 547 and 77.
 #include "common.cuh"
